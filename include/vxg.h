@@ -34,6 +34,13 @@ typedef enum vxg_epilogue {
   VXG_EP_ADD_SCALED = 2, /* y = fma(scale, v, y): residual add into a pre-filled y */
 } vxg_epilogue;
 
+/* Element types of activations (the codes vxg_model_tensor reports). */
+typedef enum vxg_dtype {
+  VXG_DT_F16 = 0,
+  VXG_DT_BF16 = 1,
+  VXG_DT_F32 = 2,
+} vxg_dtype;
+
 /* Last error message on this thread ("" if none); replaces voxrt_last_error (crates/voxrt-ffi/src/lib.rs:70). */
 const char* vxg_last_error(void);
 
@@ -124,6 +131,37 @@ vxg_status vxg_quantize_rows(const float* x, int n, int inp, int group, int8_t* 
 vxg_status vxg_ln_quant(const float* x, int n, int d, const float* g0, const float* b0, float* x_out,
                         const float* g1, const float* b1, int group, int8_t* q, float* scales, void* stream);
 
+/* Fused residual add + RMSNorm -> int8: h = fma(vs, v, x), y = (h * f32(1 / sqrt(sum h^2 / d + eps))) * gamma with the
+ * sum and the root in 64 bits, then quantisation per `group` columns as vxg_quantize_rows does it. x, v, x_res and y
+ * have the element type `dtype` and row strides ld_* in elements (>= d); gamma [d] is f32. Optional: v (NULL: h = x),
+ * x_res (receives h; may be x or v), y (receives the unquantised row), q + scales (NULL q skips quantisation; scales
+ * [n, d/group]). group is d (one scale a token, what vxg_gemm_i8 reads) or a multiple of 8 that divides d (128: what
+ * the ternary GEMMs read). d <= 32768 (else VXG_ERR_UNSUPPORTED). A NaN gives code 0 and no scale takes notice of it;
+ * x_res and y keep it. No reference counterpart (its encoder has LayerNorm only). */
+vxg_status vxg_rms_quant(const void* x, long long ld_x, const void* v, long long ld_v, float vs, int dtype, int n, int d,
+                         const float* gamma, float eps, void* x_res, long long ld_res, void* y, long long ld_y,
+                         int group, int8_t* q, float* scales, void* stream);
+
+/* vxg_quantize_rows for rows of any vxg_dtype and stride (the same codes and scales as on the values widened to f32);
+ * d and group as in vxg_rms_quant. */
+vxg_status vxg_quantize_tokens(const void* x, long long ld_x, int dtype, int n, int d, int group, int8_t* q,
+                               float* scales, void* stream);
+
+/* The values that codes stand for: out [n, inp] = q * scale, rounded once to `dtype`. Any group that divides inp. */
+vxg_status vxg_dequantize_rows(const int8_t* q, const float* scales, int n, int inp, int group, int dtype, void* out,
+                               void* stream);
+
+/* ------------------------------------------------------------------------------------------- int8 product
+ * y[t, o] = ep(f32(sum_k x[t, k] w[o, k]) * (sx[t] * sw[o]) (+ bias[o])) for t < M, o < N, the sum exact in int32: one
+ * scale a token, one an output channel. x [M, K] and w [N, K] int8 (device, contiguous, 16-byte aligned), sx [M],
+ * sw [N], bias [N] or NULL (f32), y rows of `dtype` elements with stride ld_y >= N (read first for ADD_SCALED:
+ * y = fma(ep_scale, v, y)). K a multiple of 16 below 131072 (else VXG_ERR_UNSUPPORTED); codes of -128 are allowed. The
+ * same bits for every M: a token's row does not depend on the batch it is computed in. Stands beside
+ * vxg_gemm_ternary_i8 for weights that are not ternary; no reference counterpart. */
+vxg_status vxg_gemm_i8(const int8_t* x, const float* sx, const int8_t* w, const float* sw, int M, int N, int K,
+                       vxg_epilogue ep, float ep_scale, const float* bias, int dtype, void* y, long long ld_y,
+                       void* stream);
+
 /* --------------------------------------------------------------------------------------- int8 attention
  * Relative-position MHSA core on int8 scores for a batch of utterances stacked along the token axis: utterance u
  * occupies rows [off[u], off[u] + len[u]) of qkv (row stride ld_qkv floats, q | k | v of heads * 128 each) and
@@ -139,6 +177,52 @@ vxg_status vxg_attention_i8(const float* qkv, int ld_qkv, const float* rel_k, in
                             const int* len, int n_utt, const float* bias_u, const float* bias_v, int heads,
                             int head_dim, float scaling, float* ctx, int8_t* ctx_q, float* ctx_s, void* workspace,
                             size_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------ int8 KV cache
+ * Keys and values of autoregressive decoding in a pool of pages: codes [n_pages][heads][page][head_dim] int8 and one
+ * scale per (page, head), all caller-owned device memory; a sequence's pages are listed in order in its row of a page
+ * table [n_seq, max_pages] (device int32). page is 16, 32, 64 or 128 tokens, head_dim 64 or 128 (else
+ * VXG_ERR_UNSUPPORTED); the codes are 16-byte aligned. Scales start as 0 or anything else: a page's first write sets
+ * them. No reference counterpart (its decoder is an LSTM).
+ *
+ * A batch is stacked along the token axis like the encoder's: sequence s owns rows [cu[s], cu[s + 1]) of k, v, q and
+ * out (cu: device int32 [n_seq + 1], not decreasing, cu[n_seq] <= total; rows behind the last sequence are neither read
+ * nor written). Lengths are device arrays, so calls can be captured in a CUDA graph and replayed with other lengths
+ * (make one call before the capture: it allocates the device's status word). A page id, length or offset that is out
+ * of range is not followed: its part of the work is skipped and vxg_device_status reports 0x302. */
+typedef struct vxg_kv_cache {
+  int8_t *k, *v;            /* [n_pages][heads][page][head_dim] */
+  float *k_scales, *v_scales; /* [n_pages][heads] */
+  int n_pages, heads, page, head_dim;
+} vxg_kv_cache;
+
+/* Quantise and append: k and v rows [heads * head_dim] of `dtype` with strides ld_k, ld_v (elements), to positions
+ * start[s] .. of each sequence (start: device int32, tokens cached so far). Per touched (page, head): s = max(absmax of
+ * the new finite values / 127, the page's scale if it holds earlier tokens of the sequence); earlier codes are
+ * requantised (round_ties_even(c * (old / s))) where the scale grew; new codes = clamp(round_ties_even(x * (1 / s)),
+ * +-127), NaN -> 0, +-inf -> +-127; all-zero pages have scale 0. Pages that are written must not be shared by
+ * sequences of the batch (nor appear twice in one): such a page's contents are unspecified. */
+vxg_status vxg_cache_write(const vxg_kv_cache* c, const void* k, long long ld_k, const void* v, long long ld_v, int dtype,
+                           int total, const int* table, int n_seq, int max_pages, const int* start, const int* cu,
+                           void* stream);
+
+/* Read back cu[s + 1] - cu[s] tokens from position start[s] of each sequence: k and / or v [total, heads, head_dim]
+ * (contiguous, 16-byte aligned; NULL skips one) = code * scale, rounded once to `dtype`. */
+vxg_status vxg_cache_read(const vxg_kv_cache* c, const int* table, int n_seq, int max_pages, const int* start,
+                          const int* cu, int total, int dtype, void* k, void* v, void* stream);
+
+/* Attention of the stacked queries over their sequences' cached tokens: out = softmax(scale * q k^T) v with len[s]
+ * (device int32) tokens in the cache, new ones included; query i of n sits at position len - n + i and sees positions
+ * < len, <= its own if causal, and > its own - window if window > 0; a query that sees none gives 0. q and out: rows
+ * [heads * head_dim] of `dtype` with strides ld_q, ld_out, rows 16-byte aligned; heads is a multiple of the cache's
+ * heads and query head h reads cache head h / (heads / cache heads). workspace: device memory of
+ * vxg_cache_attention_workspace_bytes(), 16-byte aligned, one per call in flight (calls that may overlap, captured
+ * graphs included, must not share it). Pages may be shared by sequences. */
+size_t vxg_cache_attention_workspace_bytes(int total, int n_seq, int heads, int kv_heads, int head_dim);
+vxg_status vxg_cache_attention(const vxg_kv_cache* c, const void* q, long long ld_q, int heads, int dtype, int total,
+                               const int* table, int n_seq, int max_pages, const int* len, const int* cu, float scale,
+                               int causal, int window, void* out, long long ld_out, void* workspace, size_t ws_bytes,
+                               void* stream);
 
 /* ------------------------------------------------------------------------------------------- conv module
  * BatchNorm(eval) folded into the bias-free depthwise conv, host to host: dw [d, 1, k] -> tap-major dw_t [k, d]

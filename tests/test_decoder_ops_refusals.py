@@ -1,0 +1,117 @@
+"""CPU: what the int8 decoder entries refuse, before anything reaches a GPU, and what they accept as empty."""
+import ctypes as C
+
+import pytest
+import torch
+
+from voxrt_b200 import _lib
+from voxrt_b200.cache import KvCache, _Desc
+from voxrt_b200.kernels import Epilogue, Int8Matrix, quantize, rms_quant
+
+P = 1 << 20  # stands for a device address: no refused or empty call follows it
+ARG, UNSUP, OK = _lib.VXG_ERR_ARG, _lib.VXG_ERR_UNSUPPORTED, _lib.VXG_OK
+
+
+def _rms(x=P, ld=64, v=None, dt=2, n=4, d=64, gamma=P, eps=1e-6, res=None, y=None, group=64, q=P, s=P, ldv=64, ldr=64):
+    return _lib.lib().vxg_rms_quant(x, ld, v, ldv, 1.0, dt, n, d, gamma, eps, res, ldr, y, 64, group, q, s, None)
+
+
+@pytest.mark.parametrize("kw,want", [
+    (dict(x=None), ARG), (dict(gamma=None), ARG), (dict(q=None, s=None), ARG), (dict(s=None), ARG), (dict(dt=3), ARG),
+    (dict(dt=-1), ARG), (dict(n=-1), ARG), (dict(d=0, group=1), ARG), (dict(ld=63), ARG), (dict(v=P, ldv=1), ARG),
+    (dict(v=P, res=P, ldr=63), ARG), (dict(res=P), ARG), (dict(eps=-1.0), ARG), (dict(eps=float("nan")), ARG),
+    (dict(group=0), ARG), (dict(group=48), ARG), (dict(group=4), UNSUP), (dict(d=32776, ld=32776, group=32776), UNSUP),
+    (dict(n=0), OK), (dict(n=0, x=None, gamma=None, q=None, s=None), OK)])
+def test_rms_quant(kw, want):
+    assert _rms(**kw) == want
+    assert want == OK or _lib.lib().vxg_last_error()
+
+
+def test_quantize_and_dequantize():
+    L = _lib.lib()
+    for a, want in (((P, 64, 2, 4, 64, 64, None, P), ARG), ((None, 64, 2, 4, 64, 64, P, P), ARG),
+                    ((P, 64, 9, 4, 64, 64, P, P), ARG), ((P, 60, 2, 4, 64, 64, P, P), ARG),
+                    ((P, 64, 2, 4, 64, 2, P, P), UNSUP), ((P, 64, 2, 0, 64, 64, P, P), OK)):
+        assert L.vxg_quantize_tokens(*a, None) == want
+    for a, want in (((P, P, 4, 64, 64, 2, None), ARG), ((P, P, 4, 64, 48, 2, P), ARG), ((P, P, 4, 64, 64, 5, P), ARG),
+                    ((P, P, -1, 64, 64, 2, P), ARG), ((P, P, 0, 64, 64, 2, P), OK)):
+        assert L.vxg_dequantize_rows(*a, None) == want
+
+
+@pytest.mark.parametrize("kw,want", [
+    (dict(x=None), ARG), (dict(x=P + 8), ARG), (dict(w=P + 4), ARG), (dict(m=-1), ARG), (dict(n=0), ARG), (dict(ep=3), ARG),
+    (dict(dt=4), ARG), (dict(ld=31), ARG), (dict(k=40), UNSUP), (dict(k=131072), UNSUP), (dict(m=0), OK)])
+def test_gemm(kw, want):
+    a = dict(x=P, sx=P, w=P, sw=P, m=4, n=32, k=64, ep=0, s=0.0, bias=None, dt=2, y=P, ld=32)
+    a.update(kw)
+    assert _lib.lib().vxg_gemm_i8(*a.values(), None) == want
+
+
+def _cache(**kw):
+    a = dict(k=P, v=P, k_scales=P, v_scales=P, n_pages=8, heads=2, page=16, head_dim=64)
+    a.update(kw)
+    return _Desc(**a)
+
+
+BAD_CACHE = [(dict(k=None), ARG), (dict(k=P + 4), ARG), (dict(v_scales=None), ARG), (dict(n_pages=0), ARG),
+             (dict(heads=0), ARG), (dict(page=8), UNSUP), (dict(page=48), UNSUP), (dict(head_dim=96), UNSUP),
+             (dict(n_pages=1 << 27), UNSUP)]
+
+
+def _write(c, k=P, ldk=128, v=P, ldv=128, dt=2, total=4, table=P, n_seq=1, width=4, start=P, cu=P):
+    return _lib.lib().vxg_cache_write(C.addressof(c), k, ldk, v, ldv, dt, total, table, n_seq, width, start, cu, None)
+
+
+def _attend(c, q=P, ld=256, heads=4, dt=2, total=4, table=P, n_seq=1, width=4, lens=P, cu=P, scale=0.1, causal=1, window=0,
+            out=P, ldo=256, ws=P, nb=1 << 30):
+    return _lib.lib().vxg_cache_attention(C.addressof(c), q, ld, heads, dt, total, table, n_seq, width, lens, cu, scale,
+                                          causal, window, out, ldo, ws, nb, None)
+
+
+def _read(c, table=P, n_seq=1, width=4, start=P, cu=P, total=4, dt=2, k=P, v=P):
+    return _lib.lib().vxg_cache_read(C.addressof(c), table, n_seq, width, start, cu, total, dt, k, v, None)
+
+
+@pytest.mark.parametrize("kw,want", BAD_CACHE)
+def test_bad_cache(kw, want):
+    c = _cache(**kw)
+    assert _write(c) == want and _attend(c) == want and _read(c) == want
+    assert _lib.lib().vxg_cache_write(None, P, 128, P, 128, 2, 4, P, 1, 4, P, P, None) == ARG
+
+
+@pytest.mark.parametrize("kw,want", [
+    (dict(table=None), ARG), (dict(cu=None), ARG), (dict(total=-1), ARG), (dict(n_seq=-1), ARG), (dict(width=0), ARG),
+    (dict(dt=7), ARG), (dict(total=0), OK), (dict(n_seq=0), OK), (dict(n_seq=0, table=None, cu=None), OK)])
+def test_bad_batch(kw, want):
+    c = _cache()
+    assert _write(c, **kw) == want and _attend(c, **kw) == want and _read(c, **kw) == want
+
+
+def test_write_read_attend():
+    c = _cache()
+    for kw in (dict(k=None), dict(v=None), dict(ldk=127), dict(ldv=1), dict(start=None)):
+        assert _write(c, **kw) == ARG
+    assert _read(c, k=None, v=None) == ARG and _read(c, k=P + 8) == ARG
+    for kw in (dict(heads=3), dict(heads=0), dict(window=-1), dict(scale=float("nan")), dict(scale=float("inf")),
+               dict(q=None), dict(ws=None), dict(ld=255), dict(ldo=128), dict(ld=257), dict(q=P + 8), dict(ws=P + 8),
+               dict(nb=16), dict(lens=None)):
+        assert _attend(c, **kw) == ARG, kw
+    L = _lib.lib()
+    assert L.vxg_cache_attention_workspace_bytes(0, 1, 4, 2, 64) == 0
+    assert L.vxg_cache_attention_workspace_bytes(4, 1, 3, 2, 64) == 0
+    assert L.vxg_cache_attention_workspace_bytes(4, 1, 4, 2, 64) > 0
+
+
+def test_python_refusals():
+    x = torch.zeros((2, 64))
+    with pytest.raises(ValueError, match="CUDA"):
+        rms_quant(x, torch.ones(64))
+    with pytest.raises(ValueError, match="divide"):
+        rms_quant(x, torch.ones(64), group=48)
+    with pytest.raises(ValueError, match="CUDA"):
+        quantize(x.half(), 64)
+    with pytest.raises(ValueError, match="int8"):
+        Int8Matrix(x, torch.ones(2))
+    with pytest.raises(ValueError, match="int8"):
+        KvCache(x, x, x, x)
+    assert Epilogue.AddScaled(2.0).kind == 2

@@ -11,7 +11,7 @@ LIB_PATH = os.path.join(HERE, "libvxg.so")
 VXG_OK, VXG_ERR_ARG, VXG_ERR_CUDA, VXG_ERR_TIMEOUT, VXG_ERR_OOM, VXG_ERR_UNSUPPORTED = range(6)
 STATUS_NAMES = {0: "OK", 1: "ERR_ARG", 2: "ERR_CUDA", 3: "ERR_TIMEOUT", 4: "ERR_OOM", 5: "ERR_UNSUPPORTED"}
 
-_P, _I, _F, _Z = C.c_void_p, C.c_int, C.c_float, C.c_size_t
+_P, _I, _F, _Z, _L = C.c_void_p, C.c_int, C.c_float, C.c_size_t, C.c_longlong
 
 # name -> (restype, argtypes): every symbol include/vxg.h declares
 SIGNATURES = {
@@ -33,6 +33,14 @@ SIGNATURES = {
     "vxg_gemm_ternary_glu": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _P, _P]),
     "vxg_quantize_rows": (_I, [_P, _I, _I, _I, _P, _P, _P]),
     "vxg_ln_quant": (_I, [_P, _I, _I, _P, _P, _P, _P, _P, _I, _P, _P, _P]),
+    "vxg_rms_quant": (_I, [_P, _L, _P, _L, _F, _I, _I, _I, _P, _F, _P, _L, _P, _L, _I, _P, _P, _P]),
+    "vxg_quantize_tokens": (_I, [_P, _L, _I, _I, _I, _I, _P, _P, _P]),
+    "vxg_dequantize_rows": (_I, [_P, _P, _I, _I, _I, _I, _P, _P]),
+    "vxg_gemm_i8": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _F, _P, _I, _P, _L, _P]),
+    "vxg_cache_write": (_I, [_P, _P, _L, _P, _L, _I, _I, _P, _I, _I, _P, _P, _P]),
+    "vxg_cache_read": (_I, [_P, _P, _I, _I, _P, _P, _I, _I, _P, _P, _P]),
+    "vxg_cache_attention_workspace_bytes": (_Z, [_I, _I, _I, _I, _I]),
+    "vxg_cache_attention": (_I, [_P, _P, _L, _I, _I, _I, _P, _I, _I, _P, _P, _F, _I, _I, _P, _L, _P, _Z, _P]),
     "vxg_fold_bn": (_I, [_P, _P, _P, _P, _P, _I, _I, _P, _P]),
     "vxg_conv_workspace_bytes": (_Z, [_I, _I]),
     "vxg_conv_glu_dw_silu_quant": (_I, [_P, _I, _P, _P, _I, _P, _P, _I, _I, _P, _P, _P, _P, _Z, _P]),

@@ -29,8 +29,8 @@ int* device_status() {
   if ((int)g_status.size() <= dev) g_status.resize(dev + 1, nullptr);
   if (!g_status[dev]) {
     int* p = nullptr;
-    if (cudaMalloc(&p, sizeof(int)) != cudaSuccess) return nullptr;
-    if (cudaMemset(p, 0, sizeof(int)) != cudaSuccess) return nullptr;
+    if (cudaMalloc(&p, 2 * sizeof(int)) != cudaSuccess) return nullptr;
+    if (cudaMemset(p, 0, 2 * sizeof(int)) != cudaSuccess) return nullptr;
     if (cudaDeviceSynchronize() != cudaSuccess) return nullptr;
     g_status[dev] = p;
   }
@@ -89,7 +89,9 @@ vxg_status make_tmap_2d_u8(CUtensorMap* map, const void* base, uint64_t rows, ui
   cuuint32_t box[2] = {box_cols, box_rows};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     set_error("cuTensorMapEncodeTiled failed (%d)", (int)r);
@@ -189,8 +191,10 @@ vxg_status vxg_device_status(int* code) {
     return VXG_ERR_CUDA;
   }
   VXG_CUDA(cudaDeviceSynchronize());
-  VXG_CUDA(cudaMemcpy(code, st, sizeof(int), cudaMemcpyDeviceToHost));
-  VXG_CUDA(cudaMemset(st, 0, sizeof(int)));
+  int w[2];
+  VXG_CUDA(cudaMemcpy(w, st, sizeof w, cudaMemcpyDeviceToHost));
+  VXG_CUDA(cudaMemset(st, 0, sizeof w));
+  *code = w[0] ? w[0] : w[1];
   return VXG_OK;
 }
 

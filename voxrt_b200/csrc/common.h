@@ -17,8 +17,9 @@ namespace vxg {
 void set_error(const char* fmt, ...);
 void clear_error();
 
-// Device status word of the current device (allocated on first use, zero-initialised). Kernels write a nonzero
-// VXG_DEV_* code on a bounded-wait timeout or an internal check failure.
+// Device status words of the current device (allocated on first use, zero-initialised). Kernels write a nonzero
+// VXG_DEV_* code to word 0 on a bounded-wait timeout or an internal check failure, and to word 1 when a device array
+// of a call held an index out of range (a word of its own: waits give up early while word 0 is set).
 int* device_status();
 
 enum : int {
@@ -29,6 +30,8 @@ enum : int {
   VXG_DEV_TIMEOUT_EPILOGUE = 0x104,
   VXG_DEV_TIMEOUT_DRAIN = 0x105,
   VXG_DEV_TIMEOUT_ATTN = 0x201,
+  VXG_DEV_TIMEOUT_CACHE_ATTN = 0x301,
+  VXG_DEV_CACHE_INDEX = 0x302,  // a page id, length or offset of a cache call was out of range (skipped, not followed)
   VXG_DEV_ATTN_PMAX = 0x202,   // a probability row's maximum was not exactly 1 (non-finite scores)
 };
 
@@ -52,7 +55,7 @@ inline vxg_status cuda_fail(cudaError_t e, const char* what) {
   } while (0)
 
 // 2D tensor map over a row-major [rows, cols] matrix of 1-byte elements with a (box_rows x box_cols) box and the
-// 128-byte swizzle (box_cols * 1 B must be 128 for that swizzle).
+// swizzle of its row: 64 columns take the 64-byte swizzle, 128 the 128-byte one.
 vxg_status make_tmap_2d_u8(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t row_stride,
                            uint32_t box_rows, uint32_t box_cols);
 

@@ -42,6 +42,66 @@ def _ptr(t):
     return None if t is None else C.c_void_p(t.data_ptr())
 
 
+_DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}  # vxg_dtype
+
+
+def _need(ok, what: str):
+    if not ok:
+        raise ValueError(what)
+
+
+def _dt(t: torch.Tensor) -> int:
+    _need(t.dtype in _DTYPES, f"element type {t.dtype} is none of float16, bfloat16, float32")
+    return _DTYPES[t.dtype]
+
+
+def _rows(t: torch.Tensor, shape, what: str) -> int:
+    """Row stride in elements of a 2-D operand whose rows are contiguous."""
+    n, d = shape
+    _need(t.dim() == 2 and tuple(t.shape) == (n, d), f"{what} has shape {tuple(t.shape)}, not {(n, d)}")
+    _need(d == 1 or t.stride(1) == 1, f"{what}'s rows must be contiguous")
+    ld = t.stride(0) if n > 1 else d
+    _need(ld >= d, f"{what}'s row stride {ld} is below its width {d}")
+    return ld
+
+
+def _on(dev: torch.device, stream, *tensors):
+    """Every operand on one GPU, and a stream of that GPU."""
+    _need(dev.type == "cuda", "operands must be CUDA tensors")
+    for t in tensors:
+        _need(t is None or t.device == dev, f"operands on {dev} and {t.device if t is not None else None}")
+    _need(stream is None or stream.device == dev, f"the stream is not {dev}'s")
+
+
+def _empty(shape, dtype, dev, stream):
+    """Memory for an output: the allocator has to know the stream that writes it."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=dev)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=dev)
+
+
+def _call(fn, dev: torch.device, stream, used, *args):
+    """A C entry on the operands' device. On a stream other than the current one, the allocator is told which operands
+    are in use there, so that memory freed by the caller meanwhile is not handed out early."""
+    if stream is None:
+        raw = torch._C._cuda_getCurrentRawStream(dev.index)
+    else:
+        raw = stream.cuda_stream
+        for t in used:
+            if t is not None:
+                t.record_stream(stream)
+    if torch.cuda.current_device() == dev.index:
+        check(fn(*args, raw))
+    else:
+        with torch.cuda.device(dev):
+            check(fn(*args, raw))
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
 class TernaryMatrix:
     """Ternary weights [out, inp] resident on the GPU in one of the kernels' formats, chosen at load time like the
     reference's Layout (packed.rs:8-27): "2bit" = 2-bit codes tiled per 128 rows x 128 columns, unpacked to int8
@@ -155,13 +215,106 @@ def gemm(w: TernaryMatrix, x: QuantAct, y: torch.Tensor, bias: torch.Tensor | No
 
 
 def quantize(x: torch.Tensor, group: int = GROUP, stream=None) -> QuantAct:
-    """QuantAct::quantize (packed.rs:302-312) on the GPU: per-(token, group) absmax/127 int8."""
-    assert x.dtype == torch.float32 and x.is_cuda and x.is_contiguous() and x.dim() == 2
-    n, inp = x.shape
-    q = torch.empty((n, inp), dtype=torch.int8, device=x.device)
-    s = torch.empty((n, inp // group), dtype=torch.float32, device=x.device)
-    check(lib().vxg_quantize_rows(_ptr(x), n, inp, group, _ptr(q), _ptr(s), _stream_ptr(stream)))
+    """QuantAct::quantize (packed.rs:302-312) on the GPU: per-(token, group) absmax/127 int8. f32, f16 or bf16 rows (any
+    row stride); group = x.shape[1] gives the one scale a token that gemm_i8 reads."""
+    if x.dtype == torch.float32 and x.is_contiguous() and x.dim() == 2 and x.shape[1] <= 8192:
+        assert x.is_cuda
+        n, inp = x.shape
+        q = torch.empty((n, inp), dtype=torch.int8, device=x.device)
+        s = torch.empty((n, inp // group), dtype=torch.float32, device=x.device)
+        check(lib().vxg_quantize_rows(_ptr(x), n, inp, group, _ptr(q), _ptr(s), _stream_ptr(stream)))
+        return QuantAct(q, s, group)
+    _on(x.device, stream, x)
+    _need(x.dim() == 2 and x.shape[1] > 0 and group > 0, "quantize takes rows")
+    n, d = x.shape
+    ld = _rows(x, (n, d), "x")
+    q = _empty((n, d), torch.int8, x.device, stream)
+    s = _empty((n, d // group), torch.float32, x.device, stream)
+    _call(lib().vxg_quantize_tokens, x.device, stream, (x,), _addr(x), ld, _dt(x), n, d, group, _addr(q), _addr(s))
     return QuantAct(q, s, group)
+
+
+def dequantize(x: QuantAct, dtype: torch.dtype = torch.float32, stream=None) -> torch.Tensor:
+    """The values that the codes stand for, q * scale, rounded once to `dtype`."""
+    dev = x.x.device
+    _on(dev, stream, x.x, x.scales)
+    _need(dtype in _DTYPES, f"element type {dtype} is none of float16, bfloat16, float32")
+    out = _empty((x.n, x.inp), dtype, dev, stream)
+    _call(lib().vxg_dequantize_rows, dev, stream, (x.x, x.scales), _addr(x.x), _addr(x.scales), x.n, x.inp, x.group,
+          _DTYPES[dtype], _addr(out))
+    return out
+
+
+def _rms(x, gamma, eps, v, vs, x_res, y, group, q, s, stream):
+    dev = x.device
+    _on(dev, stream, gamma, v, x_res, y)
+    _need(x.dim() == 2, "x must be [n, d]")
+    shape, dt = tuple(x.shape), _dt(x)
+    _need(gamma.dtype == torch.float32 and gamma.is_contiguous() and gamma.numel() == shape[1],
+          "gamma must be d contiguous float32 values")
+    ld = []
+    for t, what in ((x, "x"), (v, "v"), (x_res, "x_res"), (y, "y")):
+        _need(t is None or t.dtype == x.dtype, f"{what} must have x's element type")
+        ld.append(0 if t is None else _rows(t, shape, what))
+    _call(lib().vxg_rms_quant, dev, stream, (x, gamma, v, x_res, y), _addr(x), ld[0], _addr(v), ld[1], float(vs), dt,
+          shape[0], shape[1], _addr(gamma), float(eps), _addr(x_res), ld[2], _addr(y), ld[3], group, _addr(q), _addr(s))
+
+
+def rms_quant(x: torch.Tensor, gamma: torch.Tensor, group: int | None = None, eps: float = 1e-6,
+              v: torch.Tensor | None = None, vs: float = 1.0, x_res: torch.Tensor | None = None,
+              y: torch.Tensor | None = None, stream=None) -> QuantAct:
+    """RMSNorm -> int8 with the residual add in front, in one pass: h = x + vs * v (stored to x_res, which may be x),
+    h / sqrt(mean h^2 + eps) * gamma (stored to y, unquantised, when given), then int8 per token (group None or d: for
+    gemm_i8) or per `group` columns (128: for the ternary GEMMs). f32, f16 or bf16 rows of any stride; gamma f32."""
+    _need(x.dim() == 2 and x.shape[1] > 0, "x must be [n, d]")
+    n, d = x.shape
+    group = d if group is None else int(group)
+    _need(group > 0 and d % group == 0, f"group {group} does not divide the row width {d}")
+    _on(x.device, stream, x)
+    q = _empty((n, d), torch.int8, x.device, stream)
+    s = _empty((n, d // group), torch.float32, x.device, stream)
+    _rms(x, gamma, eps, v, vs, x_res, y, group, q, s, stream)
+    return QuantAct(q, s, group)
+
+
+def rms_norm(x: torch.Tensor, gamma: torch.Tensor, out: torch.Tensor, eps: float = 1e-6, v: torch.Tensor | None = None,
+             vs: float = 1.0, x_res: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """rms_quant without the quantisation (the norm in front of an output head) -> out (may be x if x_res is not)."""
+    _rms(x, gamma, eps, v, vs, x_res, out, 1, None, None, stream)
+    return out
+
+
+class Int8Matrix:
+    """int8 weights [out, inp] with one f32 scale per output row, resident on the GPU: gemm_i8's weights."""
+
+    def __init__(self, w: torch.Tensor, scales: torch.Tensor):
+        _need(w.dtype == torch.int8 and w.is_cuda and w.dim() == 2 and w.is_contiguous(), "weights must be [out, inp] int8")
+        self.out, self.inp = w.shape
+        _need(scales.dtype == torch.float32 and scales.device == w.device and scales.is_contiguous() and
+              scales.numel() == self.out, "one float32 scale per output row, on the weights' device")
+        self.w, self.scales = w, scales
+
+    @classmethod
+    def from_float(cls, w: torch.Tensor) -> "Int8Matrix":
+        """Float weights [out, inp] on the GPU, each row quantised to its own absmax / 127."""
+        a = quantize(w, w.shape[1])
+        return cls(a.x, a.scales.view(-1))
+
+
+def gemm_i8(w: Int8Matrix, x: QuantAct, y: torch.Tensor, bias: torch.Tensor | None = None,
+            ep: Epilogue = Epilogue.Store, stream=None) -> torch.Tensor:
+    """y[n, out] = epilogue(x w^T + bias) for int8 activations with one scale a token: exact int32 sums, then
+    sum * (token scale * channel scale). y: f32, f16 or bf16 rows of any stride, read first for AddScaled."""
+    dev = w.w.device
+    _on(dev, stream, x.x, x.scales, y, bias)
+    _need(x.inp == w.inp and x.group == x.inp, f"activations of width {x.inp} and group {x.group} for weights of width "
+          f"{w.inp}: one scale a token is wanted")
+    _need(bias is None or (bias.dtype == torch.float32 and bias.is_contiguous() and bias.numel() == w.out),
+          "bias must be `out` contiguous float32 values")
+    ld = _rows(y, (x.n, w.out), "y")
+    _call(lib().vxg_gemm_i8, dev, stream, (x.x, x.scales, w.w, w.scales, y, bias), _addr(x.x), _addr(x.scales),
+          _addr(w.w), _addr(w.scales), x.n, w.out, w.inp, ep.kind, ep.scale, _addr(bias), _dt(y), _addr(y), ld)
+    return y
 
 
 def ln_quant(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, group: int = GROUP, pre=None,
