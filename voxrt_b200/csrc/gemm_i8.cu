@@ -14,6 +14,8 @@
 #include "common.h"
 #include "dtype.cuh"
 #include "math.cuh"
+#include "ptx.cuh"
+#include "wait.cuh"
 
 namespace vxg {
 namespace i8 {
@@ -111,6 +113,274 @@ vxg_status launch_few(const Params& p, cudaStream_t st) {
   return VXG_OK;
 }
 
+// ------------------------------------------------------------------------------------------------ many tokens
+// A pair of CTAs (cta_group::2) owns a tile of 256 tokens x BN channels: each brings 128 rows of x and BN / 2 rows of w
+// into its shared memory, the leader issues M = 256 products over both, and each CTA's TMEM receives its 128 tokens'
+// int32 sums. Sharing w this way halves the operand bytes an SM reads per product, which is what limits a single CTA's
+// 128 x 256 tile. Persistent over tiles, two TMEM buffers, so a tile's epilogue runs under the next one's products.
+// Roles: warps 0-7 epilogue (TMEM lanes 32 (w % 4).., column half w / 4), warp 8 TMA producer, warp 9 MMA issuer (leader).
+namespace tc {
+
+constexpr int BM = 256, BK = 128, EPI_WARPS = 8, THREADS = (EPI_WARPS + 2) * 32;
+constexpr int GROUP_M = 8;  // token tiles that share a run of weight tiles while both stay in L2
+
+template <int BN>
+struct Cfg {
+  static constexpr uint32_t A_BYTES = 128 * BK, B_BYTES = BN / 2 * BK, STAGE = A_BYTES + B_BYTES;
+  static constexpr int STAGES = BN == 256 ? 5 : BN == 128 ? 7 : 8;
+  static constexpr uint32_t COLS = 2 * BN;             // two accumulators
+  static constexpr uint32_t XCH = STAGES * STAGE;      // [8][32][33] int32: rows that cannot be stored as vectors
+  static constexpr uint32_t SCALE = XCH + EPI_WARPS * 32 * 33 * 4;  // [2][BN] channel scales, [2][BN] bias
+  static constexpr uint32_t BARS = SCALE + 4 * BN * 4;
+  static constexpr uint32_t BYTES = BARS + (2 * STAGES + 4) * 8 + 16 + 1024;
+  static_assert(BYTES <= 232448, "shared memory budget");
+};
+
+// Tile t of the launch: runs of GROUP_M token tiles, weight tile by weight tile.
+__device__ __forceinline__ void tile_of(int t, int mt, int nt, int& m, int& n) {
+  const int per = GROUP_M * nt, g = t / per, in = t % per, rows = ::min(GROUP_M, mt - g * GROUP_M);
+  m = g * GROUP_M + in % rows;
+  n = in / rows;
+}
+
+__device__ __forceinline__ void stg32(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
+// VEC: every 32-byte run of an output row is aligned and inside or outside the row as a whole.
+template <int DT, int BN, bool VEC>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+    gemm_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const Params p,
+                   int* status) {
+  using C = Cfg<BN>;
+  using T = typename Elem<DT>::type;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::BARS);  // leader: both CTAs' bytes of a stage have landed
+  uint64_t* empty = full + C::STAGES;                            // a stage's products are done
+  uint64_t* tfull = empty + C::STAGES;                           // an accumulator is complete
+  uint64_t* tempty = tfull + 2;                                  // leader: both CTAs have read an accumulator
+  uint32_t* holder = reinterpret_cast<uint32_t*>(tempty + 2);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::STAGES; i++) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, 1);
+    }
+    for (int i = 0; i < 2; i++) {
+      mbar_init(tfull + i, 1);
+      mbar_init(tempty + i, 2 * EPI_WARPS);
+    }
+    fence_mbar_init();
+  }
+  if (warp == EPI_WARPS + 1) {
+    tmem_alloc_pair(holder, C::COLS);
+    tmem_relinquish_pair();
+  }
+  if (warp == EPI_WARPS && lane == 0) {
+    prefetch_tmap(&map_x);
+    prefetch_tmap(&map_w);
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = *holder;
+
+  const int mt = (p.M + BM - 1) / BM, nt = (p.N + BN - 1) / BN, tiles = mt * nt;
+  const int chunks = (p.K + BK - 1) / BK, pairs = gridDim.x / 2, pair = blockIdx.x / 2;
+
+  if (warp == EPI_WARPS) {
+    if (lane == 0) {
+      int it = 0;
+      bool ok = true;
+      for (int t = pair; t < tiles && ok; t += pairs) {
+        int m, n;
+        tile_of(t, mt, nt, m, n);
+        for (int c = 0; c < chunks; c++, it++) {
+          const int s = it % C::STAGES;
+          if (it >= C::STAGES && !wait_phase(empty + s, ((it / C::STAGES) - 1) & 1, status, VXG_DEV_TIMEOUT_PRODUCER)) {
+            ok = false;
+            break;
+          }
+          if (rank == 0) mbar_arrive_expect_tx(full + s, 2 * C::STAGE);
+          const uint32_t bar = map_cluster(full + s, 0);
+          uint8_t* a = smem + s * C::STAGE;
+          tma_load_2d_pair(a, &map_x, c * BK, m * BM + (int)rank * 128, bar);
+          tma_load_2d_pair(a + C::A_BYTES, &map_w, c * BK, n * BN + (int)rank * (BN / 2), bar);
+        }
+      }
+      // The copies land before the block ends: their products' commits say so; after a timeout, wait for longer than a
+      // copy can take.
+      const int last = ::min(it, (int)C::STAGES);
+      for (int i = it - last; i < it && ok; i++)
+        ok = wait_phase(empty + i % C::STAGES, (i / C::STAGES) & 1, status, VXG_DEV_TIMEOUT_DRAIN);
+      if (!ok)
+        for (const uint64_t t0 = globaltimer(); globaltimer() - t0 < 10000000ull;) __nanosleep(10000);
+    }
+  } else if (warp == EPI_WARPS + 1) {
+    if (rank == 0 && lane == 0) {
+      int it = 0, k = 0;
+      bool ok = true;
+      for (int t = pair; t < tiles && ok; t += pairs, k++) {
+        const int b = k & 1;
+        if (k >= 2 && !wait_phase(tempty + b, ((k >> 1) - 1) & 1, status, VXG_DEV_TIMEOUT_MMA)) break;
+        tc_fence_after();
+        for (int c = 0; c < chunks; c++, it++) {
+          const int s = it % C::STAGES;
+          if (!wait_phase(full + s, (it / C::STAGES) & 1, status, VXG_DEV_TIMEOUT_MMA)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t ad = umma_desc_sw128(smem_u32(smem + s * C::STAGE));
+          const uint64_t bd = umma_desc_sw128(smem_u32(smem + s * C::STAGE + C::A_BYTES));
+#pragma unroll
+          for (int j = 0; j < BK / 32; j++)
+            mma_i8_pair(tmem + b * BN, ad + 2 * j, bd + 2 * j, idesc_i8(BM, BN), (c | j) != 0 ? 1u : 0u);
+          mma_commit_pair(empty + s);
+        }
+        if (ok) mma_commit_pair(tfull + b);
+      }
+    }
+  } else {
+    const int q = warp & 3, half = warp >> 2, tid = threadIdx.x;
+    float* sw_s = reinterpret_cast<float*>(smem + C::SCALE);
+    int* xch = reinterpret_cast<int*>(smem + C::XCH) + warp * 32 * 33;
+    T* y = static_cast<T*>(p.y);
+    int k = 0;
+    bool ok = true;
+    for (int t = pair; t < tiles; t += pairs, k++) {
+      const int b = k & 1;
+      int m, n;
+      tile_of(t, mt, nt, m, n);
+      const int n0 = n * BN;
+      float* sw = sw_s + b * BN;
+      float* bs = sw_s + (2 + b) * BN;
+      for (int i = tid; i < BN; i += EPI_WARPS * 32) {
+        sw[i] = n0 + i < p.N ? __ldg(p.sw + n0 + i) : 0.0f;
+        bs[i] = p.bias && n0 + i < p.N ? __ldg(p.bias + n0 + i) : 0.0f;
+      }
+      named_bar_sync(1, EPI_WARPS * 32);  // also: nobody is still at the tile that used this half two tiles ago
+      const int row0 = m * BM + (int)rank * 128 + q * 32, row = row0 + lane;
+      const float sx = row < p.M ? __ldg(p.sx + row) : 0.0f;
+      // a warp that gave up goes on to meet the others' barriers, without reading or writing anything more
+      ok = ok && wait_phase(tfull + b, (k >> 1) & 1, status, VXG_DEV_TIMEOUT_EPILOGUE);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) continue;
+      tc_fence_after();
+#pragma unroll 1
+      for (int c0 = half * (BN / 2); c0 < (half + 1) * (BN / 2); c0 += 32) {
+        uint32_t r[32];
+        tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(b * BN + c0), r);
+        tmem_wait_ld();
+        if (c0 + 32 == (half + 1) * (BN / 2)) {  // the warp's last read of this accumulator
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(map_cluster(tempty + b, 0));
+        }
+        if (VEC) {
+          constexpr int E = DT == VXG_DT_F32 ? 8 : 16;  // elements of 32 bytes
+          if (row < p.M) {
+            T* yo = y + (size_t)row * p.ld_y + n0 + c0;
+#pragma unroll
+            for (int j = 0; j < 32; j += E) {
+              if (n0 + c0 + j < p.N) {
+                float v[E];
+                if (p.ep == VXG_EP_ADD_SCALED) {
+#pragma unroll
+                  for (int e = 0; e < E; e += 8) {
+                    float o8[8];
+                    load8<DT>(yo + j + e, o8);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) v[e + i] = o8[i];
+                  }
+                }
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                  v[e] = finish(p, (int)r[j + e], sx, sw[c0 + j + e], bs[c0 + j + e], p.ep == VXG_EP_ADD_SCALED ? v[e] : 0.0f);
+                uint32_t o[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                  if constexpr (DT == VXG_DT_F32) o[e] = __float_as_uint(v[e]);
+                  else o[e] = narrow2<DT>(v[2 * e], v[2 * e + 1]);
+                }
+                stg32(yo + j, o);
+              }
+            }
+          }
+        } else {
+          // rows of any alignment: through shared memory, so that a store covers consecutive columns of one row
+#pragma unroll
+          for (int j = 0; j < 32; j++) xch[lane * 33 + j] = (int)r[j];
+          __syncwarp();
+          const int col = n0 + c0 + lane;
+          const float swc = sw[c0 + lane], bsc = bs[c0 + lane];
+          for (int i = 0; i < 32; i++) {
+            const float sxi = __shfl_sync(0xffffffffu, sx, i);
+            if (row0 + i < p.M && col < p.N) {
+              T* yo = y + (size_t)(row0 + i) * p.ld_y + col;
+              *yo = Elem<DT>::narrow(finish(p, xch[i * 33 + lane], sxi, swc, bsc,
+                                            p.ep == VXG_EP_ADD_SCALED ? Elem<DT>::widen(*yo) : 0.0f));
+            }
+          }
+          __syncwarp();
+        }
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // neither CTA leaves while the other may still signal its barriers
+  if (warp == EPI_WARPS + 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, C::COLS);
+  }
+}
+
+template <int DT, int BN>
+vxg_status launch(const Params& p, cudaStream_t st) {
+  int* status = device_status();
+  VXG_ARG(status, "no CUDA device");
+  CUtensorMap mx, mw;
+  vxg_status r = make_tmap_2d_u8(&mx, p.x, (uint64_t)p.M, (uint64_t)p.K, (uint64_t)p.K, 128, BK);
+  if (r == VXG_OK) r = make_tmap_2d_u8(&mw, p.w, (uint64_t)p.N, (uint64_t)p.K, (uint64_t)p.K, BN / 2, BK);
+  if (r != VXG_OK) return r;
+  const long long tiles = (long long)((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
+  if (tiles > 0x3FFFFFFF) {
+    set_error("M = %d x N = %d is more than one launch covers", p.M, p.N);
+    return VXG_ERR_UNSUPPORTED;
+  }
+  const int e = DT == VXG_DT_F32 ? 8 : 16;
+  const bool vec = p.N % e == 0 && (((uintptr_t)p.y | (uintptr_t)(p.ld_y * (long long)dtype_bytes(DT))) & 31) == 0;
+  const void* k = vec ? (const void*)gemm_tc_kernel<DT, BN, true> : (const void*)gemm_tc_kernel<DT, BN, false>;
+  if ((r = smem_attr(k, (int)Cfg<BN>::BYTES)) != VXG_OK) return r;
+  const int grid = 2 * (int)std::min<long long>(tiles, sm_count() / 2);
+  void* args[] = {&mx, &mw, const_cast<Params*>(&p), &status};
+  VXG_CUDA(cudaLaunchKernel(k, dim3(grid), dim3(THREADS), args, Cfg<BN>::BYTES, st));
+  note_launch();
+  VXG_CUDA(cudaGetLastError());
+  return VXG_OK;
+}
+
+}  // namespace tc
+
+static int pick_bn(const Params& p, int pairs) {
+  int best = 256;
+  long long cost = 0;
+  for (int bn = 256; bn >= 64; bn /= 2) {
+    const long long tiles = (long long)((p.M + tc::BM - 1) / tc::BM) * ((p.N + bn - 1) / bn);
+    const long long c = (tiles + pairs - 1) / pairs * (bn + 64);
+    if (bn == 256 || c < cost) best = bn, cost = c;
+  }
+  return best;
+}
+
 }  // namespace i8
 }  // namespace vxg
 
@@ -136,9 +406,15 @@ extern "C" vxg_status vxg_gemm_i8(const int8_t* x, const float* sx, const int8_t
   with_dtype(dtype, [&](auto tag) {
     constexpr int DT = decltype(tag)::value;
     cudaStream_t st = (cudaStream_t)stream;
-    r = M <= 8 ? i8::launch_few<DT, 1>(p, st)
-        : M <= 16 ? i8::launch_few<DT, 2>(p, st)
-        : M <= 32 ? i8::launch_few<DT, 4>(p, st) : i8::launch_few<DT, 8>(p, st);
+    if (M <= 64) {
+      r = M <= 8 ? i8::launch_few<DT, 1>(p, st)
+          : M <= 16 ? i8::launch_few<DT, 2>(p, st)
+          : M <= 32 ? i8::launch_few<DT, 4>(p, st) : i8::launch_few<DT, 8>(p, st);
+    } else {
+      const int bn = i8::pick_bn(p, sm_count() / 2);
+      r = bn == 256 ? i8::tc::launch<DT, 256>(p, st)
+          : bn == 128 ? i8::tc::launch<DT, 128>(p, st) : i8::tc::launch<DT, 64>(p, st);
+    }
   });
   return r;
 }
