@@ -218,7 +218,7 @@ vxg_status vxg_cache_read(const vxg_kv_cache* c, const int* table, int n_seq, in
  * heads and query head h reads cache head h / (heads / cache heads). workspace: device memory of
  * vxg_cache_attention_workspace_bytes(), 16-byte aligned, one per call in flight (calls that may overlap, captured
  * graphs included, must not share it). Pages may be shared by sequences. */
-size_t vxg_cache_attention_workspace_bytes(int total, int n_seq, int heads, int kv_heads, int head_dim);
+size_t vxg_cache_attention_workspace_bytes(int total, int n_seq, int heads, int kv_heads, int head_dim, int dtype);
 vxg_status vxg_cache_attention(const vxg_kv_cache* c, const void* q, long long ld_q, int heads, int dtype, int total,
                                const int* table, int n_seq, int max_pages, const int* len, const int* cu, float scale,
                                int causal, int window, void* out, long long ld_out, void* workspace, size_t ws_bytes,

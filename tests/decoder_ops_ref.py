@@ -85,7 +85,8 @@ class Cache:
 def attend(cache, q, table, lens, cu, scale, causal, window, dtype):
     """(out, bound) in 64 bits; `bound` is how far the library's result may be off, element by element.
 
-    Per probability: f16 rounding, 11 significant bits and so at most 2^-11 (f32 queries: two parts, 2^-22) and the error of its score, twice (numerator and
+    Per probability: f16 rounding, 11 significant bits and so at most 2^-11, and the same for a value times its scale where
+    the tiles are large, 2^-10 together (f32 queries: two parts, 2^-22), and the error of its score, twice (numerator and
     denominator). A score is a sum of hd exact products in f32, in the tensor cores' order: at most (hd + 8) half-steps
     of truncation (2^-23) of sum |q k|; exp2 and the scale products add less than 2^-20 relative for the scores' size met
     here. A probability is rounded in units of 2^-14 of the largest value scale `ref`: f16's finest step 2^-24 there puts
@@ -94,7 +95,7 @@ def attend(cache, q, table, lens, cu, scale, causal, window, dtype):
     rows, heads, hd = q.shape
     share = heads // cache.heads
     out, bound = np.zeros((rows, heads, hd)), np.zeros((rows, heads, hd))
-    prob = 2.0 ** -22 if dtype == torch.float32 else 2.0 ** -11
+    prob = 2.0 ** -22 if dtype == torch.float32 else 2.0 ** -10
     for s in range(len(lens)):
         L, n = int(lens[s]), int(cu[s + 1] - cu[s])
         if n == 0 or L == 0:

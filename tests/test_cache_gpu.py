@@ -175,6 +175,12 @@ CASES = [  # (page, hd, kv heads, query heads, lengths, new tokens, causal, wind
     (64, 64, 1, 3, [90, 20], [90, 3], False, 25),
     (32, 64, 2, 2, [5, 0, 64], [9, 4, 70], True, 0),      # more queries than cached tokens: rows without a key
     (128, 128, 1, 32, [1000], [1], True, 0),
+    (16, 128, 2, 8, [300, 700, 90], [300, 130, 1], True, 0),   # tiles of many rows, with a single-token sequence among them
+    (64, 64, 1, 4, [1000], [200], True, 130),
+    (32, 128, 1, 2, [250, 0], [250, 3], False, 0),
+    (128, 128, 2, 4, [50, 200], [200, 200], True, 0),          # most rows of the first sequence see no key
+    (128, 64, 3, 3, [513, 129], [257, 128], True, 0),
+    (64, 128, 1, 7, [700], [101], False, 300),
     (64, 128, 8, 8, [2500], [1], True, 0),                # one sequence over many shares
 ]
 

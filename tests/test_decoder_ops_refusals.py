@@ -97,9 +97,9 @@ def test_write_read_attend():
                dict(nb=16), dict(lens=None)):
         assert _attend(c, **kw) == ARG, kw
     L = _lib.lib()
-    assert L.vxg_cache_attention_workspace_bytes(0, 1, 4, 2, 64) == 0
-    assert L.vxg_cache_attention_workspace_bytes(4, 1, 3, 2, 64) == 0
-    assert L.vxg_cache_attention_workspace_bytes(4, 1, 4, 2, 64) > 0
+    assert L.vxg_cache_attention_workspace_bytes(0, 1, 4, 2, 64, 2) == 0
+    assert L.vxg_cache_attention_workspace_bytes(4, 1, 3, 2, 64, 2) == 0
+    assert L.vxg_cache_attention_workspace_bytes(4, 1, 4, 2, 64, 2) > 0
 
 
 def test_python_refusals():

@@ -39,7 +39,7 @@ SIGNATURES = {
     "vxg_gemm_i8": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _F, _P, _I, _P, _L, _P]),
     "vxg_cache_write": (_I, [_P, _P, _L, _P, _L, _I, _I, _P, _I, _I, _P, _P, _P]),
     "vxg_cache_read": (_I, [_P, _P, _I, _I, _P, _P, _I, _I, _P, _P, _P]),
-    "vxg_cache_attention_workspace_bytes": (_Z, [_I, _I, _I, _I, _I]),
+    "vxg_cache_attention_workspace_bytes": (_Z, [_I, _I, _I, _I, _I, _I]),
     "vxg_cache_attention": (_I, [_P, _P, _L, _I, _I, _I, _P, _I, _I, _P, _P, _F, _I, _I, _P, _L, _P, _Z, _P]),
     "vxg_fold_bn": (_I, [_P, _P, _P, _P, _P, _I, _I, _P, _P]),
     "vxg_conv_workspace_bytes": (_Z, [_I, _I]),

@@ -4,12 +4,11 @@ so a decode step can be captured in a CUDA graph and replayed as the sequences g
 from __future__ import annotations
 
 import ctypes as C
-import math
 
 import torch
 
 from ._lib import lib
-from .kernels import _DTYPES, _addr, _call, _dt, _empty, _need, _on
+from .kernels import _DTYPES, _call, _dt, _gpu, _like
 
 
 class _Desc(C.Structure):  # vxg_kv_cache
@@ -19,10 +18,14 @@ class _Desc(C.Structure):  # vxg_kv_cache
 
 def _stacked(t: torch.Tensor, heads: int, hd: int, what: str) -> int:
     """Row stride of a stacked [rows, heads, head_dim] operand whose rows are contiguous."""
-    _need(t.dim() == 3 and t.shape[1] == heads and t.shape[2] == hd,
-          f"{what} has shape {tuple(t.shape)}, not (rows, {heads}, {hd})")
-    _need(t.stride(2) == 1 and (heads == 1 or t.stride(1) == hd), f"{what}'s rows must be contiguous")
-    return t.stride(0) if t.shape[0] > 1 else heads * hd
+    shape = t.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != hd:
+        raise ValueError(f"{what} has shape {tuple(shape)}, not (rows, {heads}, {hd})")
+    if t.is_contiguous():
+        return heads * hd
+    if t.stride(2) != 1 or (heads > 1 and t.stride(1) != hd):
+        raise ValueError(f"{what}'s rows must be contiguous")
+    return t.stride(0) if shape[0] > 1 else heads * hd
 
 
 class KvCache:
@@ -31,13 +34,13 @@ class KvCache:
     [n_seq, max_pages] (int32) lists each sequence's pages in order, entries behind its last page are not read."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, ks: torch.Tensor, vs: torch.Tensor):
-        _need(k.dim() == 4 and k.dtype == torch.int8 and k.is_contiguous() and k.is_cuda,
-              "k must be a contiguous int8 CUDA tensor [n_pages, heads, page, head_dim]")
-        _need(v.shape == k.shape and v.dtype == torch.int8 and v.is_contiguous() and v.device == k.device,
-              "v must be like k")
+        if k.dim() != 4 or k.dtype != torch.int8 or not k.is_contiguous() or k.get_device() < 0:
+            raise ValueError("k must be a contiguous int8 CUDA tensor [n_pages, heads, page, head_dim]")
+        if v.shape != k.shape or v.dtype != torch.int8 or not v.is_contiguous() or v.device != k.device:
+            raise ValueError("v must be like k")
         for t in (ks, vs):
-            _need(t.shape == k.shape[:2] and t.dtype == torch.float32 and t.is_contiguous() and t.device == k.device,
-                  "scales must be contiguous float32 [n_pages, heads] on the codes' device")
+            if t.shape != k.shape[:2] or t.dtype != torch.float32 or not t.is_contiguous() or t.device != k.device:
+                raise ValueError("scales must be contiguous float32 [n_pages, heads] on the codes' device")
         self.k, self.v, self.ks, self.vs = k, v, ks, vs
         self.n_pages, self.heads, self.page, self.head_dim = k.shape
         self._desc = _Desc(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), *k.shape)
@@ -51,37 +54,42 @@ class KvCache:
         return cls(*codes, *scales)
 
     def _batch(self, table, a, cu, stream, *more):
-        _on(self.k.device, stream, table, a, cu, *more)
-        for t, what in ((table, "the page table"), (a, "lengths"), (cu, "offsets")):
-            _need(t.dtype == torch.int32 and t.is_contiguous(), f"{what} must be contiguous int32")
-        _need(table.dim() == 2 and a.shape == (table.shape[0],) and cu.shape == (table.shape[0] + 1,),
-              f"page table {tuple(table.shape)}, lengths {tuple(a.shape)} and offsets {tuple(cu.shape)} do not belong "
-              "to one batch")
-        return table.shape
-
-    def _mine(self):
-        return (self.k, self.v, self.ks, self.vs)
+        """(GPU, sequences, pages of a table row) of a batch whose lengths and offsets are a and cu."""
+        idx = _gpu(stream, self.k, table, a, cu, *more)
+        for t in (table, a, cu):
+            if t.dtype != torch.int32 or not t.is_contiguous():
+                raise ValueError("the page table, lengths and offsets must be contiguous int32")
+        n_seq, width = table.shape if table.dim() == 2 else (-1, 0)
+        if a.shape != (n_seq,) or cu.shape != (n_seq + 1,):
+            raise ValueError(f"page table {tuple(table.shape)}, lengths {tuple(a.shape)} and offsets {tuple(cu.shape)} do "
+                             "not belong to one batch")
+        return idx, n_seq, width
 
     def write(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, start: torch.Tensor, cu: torch.Tensor,
               stream=None) -> None:
         """Quantise and append k and v [rows, heads, head_dim] (f32, f16 or bf16, any row stride): rows cu[s] .. cu[s+1]
         go to positions start[s] .. of sequence s. A started page's scale grows when it has to, and its earlier codes
         with it. Pages that are written must belong to one sequence each."""
-        n_seq, width = self._batch(table, start, cu, stream, k, v)
-        _need(k.dtype == v.dtype and k.shape == v.shape, "k and v must be alike")
-        ld_k, ld_v = _stacked(k, self.heads, self.head_dim, "k"), _stacked(v, self.heads, self.head_dim, "v")
-        _call(lib().vxg_cache_write, self.k.device, stream, (k, v, table, start, cu) + self._mine(), self._ref, _addr(k),
-              ld_k, _addr(v), ld_v, _dt(k), k.shape[0], _addr(table), n_seq, width, _addr(start), _addr(cu))
+        idx, n_seq, width = self._batch(table, start, cu, stream, k, v)
+        if k.dtype != v.dtype or k.shape != v.shape:
+            raise ValueError("k and v must be alike")
+        heads, hd = self.heads, self.head_dim
+        ld_k, ld_v = _stacked(k, heads, hd, "k"), _stacked(v, heads, hd, "v")
+        _call(lib().vxg_cache_write, idx, stream, (k, v, table, start, cu, self.k, self.v, self.ks, self.vs), self._ref,
+              k.data_ptr(), ld_k, v.data_ptr(), ld_v, _dt(k), k.shape[0], table.data_ptr(), n_seq, width,
+              start.data_ptr(), cu.data_ptr())
 
     def read(self, table: torch.Tensor, start: torch.Tensor, cu: torch.Tensor, total: int,
              dtype: torch.dtype = torch.float32, stream=None):
         """The values of cu[s+1] - cu[s] tokens from position start[s] of each sequence: k, v [total, heads, head_dim]."""
-        n_seq, width = self._batch(table, start, cu, stream)
-        _need(dtype in _DTYPES, f"element type {dtype} is none of float16, bfloat16, float32")
-        dev = self.k.device
-        k, v = (_empty((total, self.heads, self.head_dim), dtype, dev, stream) for _ in range(2))
-        _call(lib().vxg_cache_read, dev, stream, (table, start, cu) + self._mine(), self._ref, _addr(table), n_seq, width,
-              _addr(start), _addr(cu), total, _DTYPES[dtype], _addr(k), _addr(v))
+        idx, n_seq, width = self._batch(table, start, cu, stream)
+        if dtype not in _DTYPES:
+            raise ValueError(f"element type {dtype} is none of float16, bfloat16, float32")
+        shape = (total, self.heads, self.head_dim)
+        k, v = _like(self.k, shape, dtype, stream), _like(self.k, shape, dtype, stream)
+        _call(lib().vxg_cache_read, idx, stream, (table, start, cu, self.k, self.v, self.ks, self.vs), self._ref,
+              table.data_ptr(), n_seq, width, start.data_ptr(), cu.data_ptr(), total, _DTYPES[dtype], k.data_ptr(),
+              v.data_ptr())
         return k, v
 
     def attend(self, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, cu: torch.Tensor,
@@ -91,25 +99,25 @@ class KvCache:
         lengths[s] tokens, the rows' own included (write before attending). Query i of n sits at position
         lengths - n + i; it sees positions up to its own (causal) and, with window > 0, the last `window` of them. heads
         is a multiple of the cache's; neighbouring query heads share a cache head. scale defaults to head_dim ** -0.5."""
-        heads = q.shape[1] if q.dim() == 3 else 0
-        _need(heads > 0 and heads % self.heads == 0, f"{heads} query heads for {self.heads} key / value heads")
-        n_seq, width = self._batch(table, lengths, cu, stream, q, out)
-        dev = self.k.device
-        ld_q = _stacked(q, heads, self.head_dim, "q")
+        idx, n_seq, width = self._batch(table, lengths, cu, stream, q, out)
+        if torch.cuda.current_device() != idx:  # the workspace's size is the current device's
+            with torch.cuda.device(idx):
+                return self.attend(q, table, lengths, cu, scale, causal, window, out, stream)
+        heads, hd = q.shape[1] if q.dim() == 3 else 0, self.head_dim
+        if heads == 0 or heads % self.heads != 0:
+            raise ValueError(f"{heads} query heads for {self.heads} key / value heads")
+        dt, ld_q = _dt(q), _stacked(q, heads, hd, "q")
         if out is None:
-            out = _empty(tuple(q.shape), q.dtype, dev, stream)
-        _need(out.dtype == q.dtype and out.shape == q.shape, "out must be like q")
-        ld_out = _stacked(out, heads, self.head_dim, "out")
+            out = _like(q, q.shape, q.dtype, stream)
+        elif out.dtype != q.dtype or out.shape != q.shape:
+            raise ValueError("out must be like q")
+        ld_out = _stacked(out, heads, hd, "out")
         total = q.shape[0]
         # the workspace is this call's own: captured graphs and streams never share one
-        if torch.cuda.current_device() == dev.index:
-            nb = lib().vxg_cache_attention_workspace_bytes(total, n_seq, heads, self.heads, self.head_dim)
-        else:
-            with torch.cuda.device(dev):
-                nb = lib().vxg_cache_attention_workspace_bytes(total, n_seq, heads, self.heads, self.head_dim)
-        ws = _empty((nb,), torch.uint8, dev, stream)
-        _call(lib().vxg_cache_attention, dev, stream, (q, table, lengths, cu, out) + self._mine(), self._ref, _addr(q),
-              ld_q, heads, _dt(q), total, _addr(table), n_seq, width, _addr(lengths), _addr(cu),
-              float(scale) if scale is not None else 1.0 / math.sqrt(self.head_dim), int(causal), int(window),
-              _addr(out), ld_out, _addr(ws), nb)
+        nb = lib().vxg_cache_attention_workspace_bytes(total, n_seq, heads, self.heads, hd, dt)
+        ws = _like(q, (nb,), torch.uint8, stream)
+        _call(lib().vxg_cache_attention, idx, stream, (q, table, lengths, cu, out, self.k, self.v, self.ks, self.vs),
+              self._ref, q.data_ptr(), ld_q, heads, dt, total, table.data_ptr(), n_seq, width, lengths.data_ptr(),
+              cu.data_ptr(), scale if scale is not None else hd ** -0.5, causal, window, out.data_ptr(), ld_out,
+              ws.data_ptr(), nb)
         return out

@@ -27,10 +27,7 @@
 #include <algorithm>
 
 #include "common.h"
-#include "dtype.cuh"
-#include "kv_cache.cuh"
-#include "ptx.cuh"
-#include "wait.cuh"
+#include "cached_attention.cuh"
 
 namespace vxg {
 namespace catt {
@@ -38,133 +35,6 @@ namespace catt {
 constexpr int BK = 64;       // keys per block
 constexpr int CONS = 4;      // consumer warps
 constexpr int THREADS = (CONS + 1) * 32;
-constexpr int MAX_PIECES = 2;  // partial results a CTA can leave: its first and its last
-
-struct Params {
-  vxg_kv_cache c;
-  const void* q;
-  void* out;
-  long long ld_q, ld_out;
-  const int* table;
-  const int* len;
-  const int* cu;
-  float* part;      // [grid][2][MT][HD + 2]
-  long long* rec;   // [grid][8]: begin, first unit and end of the tile it lies in, slot of the batch, KV head
-  int* status;
-  int n_seq, max_pages, total, heads, share, window, causal, slots, grid;
-  float scale_log2;
-};
-
-// One tile: MT rows of sequence s; `cost` units per KV head (0: no such tile, 1 where no key is visible).
-struct Tile {
-  int s, n, L, q0;       // sequence, its queries, its length, its first stacked row
-  int r0, rows;          // first (query, head) row and their number
-  int kmin, kmax;        // keys [kmin, kmax) that any of its rows sees
-  int blk0, nblk, cost;
-};
-
-__device__ __forceinline__ long long slot_base(const Params& p, int s, int MT) {
-  return (long long)__ldg(p.cu + s) * p.share / MT + s;
-}
-
-__device__ __forceinline__ int find_seq(const Params& p, long long slot, int MT) {
-  int lo = 0, hi = p.n_seq;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (slot_base(p, mid, MT) <= slot) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
-
-// The tile of a slot; s is a lower bound of its sequence and moves up to it.
-__device__ __forceinline__ Tile tile_at(const Params& p, long long slot, int& s, int MT) {
-  while (s + 1 < p.n_seq && slot_base(p, s + 1, MT) <= slot) s++;
-  Tile t;
-  t.s = s;
-  t.q0 = __ldg(p.cu + s);
-  const long long n = (long long)__ldg(p.cu + s + 1) - t.q0;
-  t.n = (int)n;
-  t.L = __ldg(p.len + s);
-  t.cost = 0;
-  t.nblk = 0;
-  const long long k = slot - slot_base(p, s, MT);
-  if (n == 0 || k < 0) return t;
-  if (n < 0 || t.q0 < 0 || t.q0 + n > p.total || t.L < 0 || t.L > (long long)p.max_pages * p.c.page) {
-    atomicCAS(p.status + 1, 0, VXG_DEV_CACHE_INDEX);
-    return t;
-  }
-  const long long r0 = k * MT, all = n * p.share;
-  if (r0 >= all) return t;
-  t.r0 = (int)r0;
-  t.rows = (int)(all - r0 < MT ? all - r0 : MT);
-  const int i0 = (int)(r0 / p.share), i1 = (int)((r0 + t.rows - 1) / p.share);
-  t.kmax = p.causal ? ::max(0, ::min(t.L, t.L - t.n + i1 + 1)) : t.L;
-  t.kmin = 0;
-  if (p.window > 0) t.kmin = (int)::max(0LL, (long long)t.L - t.n + i0 - p.window + 1);
-  t.blk0 = t.kmin / BK;
-  t.nblk = t.kmax > t.kmin ? (t.kmax + BK - 1) / BK - t.blk0 : 0;
-  t.cost = ::max(1, t.nblk);
-  return t;
-}
-
-// What a CTA works on: keys blk0 + off .. of tile t for KV head h, `left` units of its share to go (0: done).
-struct Piece {
-  Tile t;
-  long long slot, left;
-  int h, off, first;
-  __device__ __forceinline__ int take() const { return (int)::min((long long)(t.cost - off), left); }
-  // Moves on to the next piece. Ends the share where no tile is left, whatever the lengths have become meanwhile.
-  __device__ __forceinline__ void next(const Params& p, int MT) {
-    left -= take();
-    off = 0;
-    first = 0;
-    if (left > 0 && ++h == p.c.heads) {
-      h = 0;
-      int s = t.s;
-      do {
-        if (++slot >= p.slots) {
-          left = 0;
-          return;
-        }
-        t = tile_at(p, slot, s, MT);
-      } while (t.cost == 0);
-    }
-  }
-};
-
-__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// Two int8 codes in bytes 0 and 2 of w -> two f16. Flipping a code's sign bit adds 128, and 0x64 above it makes the
-// f16 1024 + 128 + code, exactly.
-__device__ __forceinline__ uint32_t codes_to_f16(uint32_t w) {
-  const uint32_t biased = (w & 0x00FF00FFu) ^ 0x64806480u;
-  const uint32_t off = 0x64806480u;  // 1152, 1152
-  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&biased), *reinterpret_cast<const __half2*>(&off));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-
-__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-// the part of (a, b) that pack_f16 leaves out
-__device__ __forceinline__ uint32_t pack_rest(float a, float b, uint32_t hi) {
-  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-  return pack_f16(a - f.x, b - f.y);
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
 template <int HD, int MT>
 struct Layout {
   static constexpr uint32_t TILE = BK * HD;      // bytes of one block's keys or values
@@ -200,7 +70,6 @@ __global__ void __launch_bounds__(THREADS, 2)
   float* scales_s = reinterpret_cast<float*>(smem + Lay::SCALES);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + Lay::BARS);
   uint64_t* empty = full + Lay::STAGES;
-  __shared__ long long warp_tot[CONS + 1];
   __shared__ Piece first_s;  // the share's first piece
   __shared__ Piece piece_s;  // few rows: the consumers' next one
   __shared__ int fail;
@@ -213,73 +82,19 @@ __global__ void __launch_bounds__(THREADS, 2)
       mbar_init(empty + i, CONS);
     }
     fence_mbar_init();
-    first_s.left = 0;
     fail = 0;
   }
 
-  // ---- the share: each thread sums the costs of a run of slots, one scan over the block, then the thread in whose run
-  // the share begins walks it again
-  const int per = (p.slots + THREADS - 1) / THREADS;
-  const int sl0 = ::min(p.slots, tid * per), sl1 = ::min(p.slots, sl0 + per);
-  const int first_seq = sl0 < sl1 ? find_seq(p, sl0, MT) : 0;
-  long long mine = 0;
-  {
-    int s = first_seq;
-    for (int i = sl0; i < sl1; i++) mine += tile_at(p, i, s, MT).cost;
-  }
-  long long incl = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
-  }
-  if (lane == 31) warp_tot[warp] = incl;
-  __syncthreads();
-  long long before = 0, units = 0;
-#pragma unroll
-  for (int i = 0; i <= CONS; i++) {
-    if (i < warp) before += warp_tot[i];
-    units += warp_tot[i];
-  }
-  before += incl - mine;
-  units *= KV;
-  const long long parts = ::min((long long)gridDim.x, units);  // at least one unit a CTA
-  if (blockIdx.x < parts) {
-    const long long begin = units * blockIdx.x / parts, end = units * (blockIdx.x + 1) / parts;
-    if (begin >= before * KV && begin < (before + mine) * KV) {
-      long long at = before;
-      int s = first_seq;
-      for (int i = sl0; i < sl1; i++) {
-        const Tile t = tile_at(p, i, s, MT);
-        if (begin < (at + t.cost) * KV) {
-          const long long in = begin - at * KV;
-          first_s.t = t;
-          first_s.slot = i;
-          first_s.h = (int)(in / t.cost);
-          first_s.off = (int)(in % t.cost);
-          first_s.left = end - begin;
-          first_s.first = 1;
-          long long* r = p.rec + blockIdx.x * 8;
-          r[0] = begin, r[1] = begin - first_s.off, r[2] = r[1] + t.cost, r[3] = i, r[4] = first_s.h, r[5] = end;
-          break;
-        }
-        at += t.cost;
-      }
-    }
-  }
-  __syncthreads();
+  find_share<THREADS, MT, BK>(p, &first_s);
   Piece w = first_s;
-  if (w.left == 0) {  // more CTAs than units
-    if (tid == 0) p.rec[blockIdx.x * 8] = -1;
-    return;
-  }
+  if (w.left == 0) return;
 
   if (warp == CONS) {
     // ------------------------------------------------------------------------------------------------ producer
     const int box = ::min(P, BK);
     int it = 0;
     bool ok = true;
-    for (; w.left > 0 && ok; w.next(p, MT)) {
+    for (; w.left > 0 && ok; w.next(p, MT, BK)) {
       const Tile& t = w.t;
       const int take = w.take(), h = w.h, off = w.off;
       if (t.nblk > 0) {
@@ -551,7 +366,7 @@ __global__ void __launch_bounds__(THREADS, 2)
       named_bar_sync(1, CONS * 32);
       if (tid == 0) {  // one thread walks on for all of them, so that they always agree on the barriers to come
         Piece n = w;
-        n.next(p, MT);
+        n.next(p, MT, BK);
         piece_s = n;
       }
       for (int r = warp; r < t.rows; r += CONS) {
@@ -617,86 +432,36 @@ __global__ void __launch_bounds__(THREADS, 2)
       w = piece_s;
     } else {
       if (!ok) return;
-      w.next(p, MT);
+      w.next(p, MT, BK);
     }
   }
 }
 
-// Joins the partial results of the tiles that span shares: block b looks at the tile in which share b begins, unless an
-// earlier share begins inside it too; a warp takes a row.
-template <int HD, int DT, int MT>
-__global__ void __launch_bounds__(128) join_kernel(const Params p) {
-  using T = typename Elem<DT>::type;
-  constexpr int N = HD / 32;
-  const int b = blockIdx.x + 1, lane = threadIdx.x & 31, r = blockIdx.y * 4 + (threadIdx.x >> 5);
-  const long long* rec = p.rec + (size_t)b * 8;
-  const long long begin = rec[0];
-  if (begin < 0) return;
-  const long long u0 = rec[1], u1 = rec[2], prev = rec[-8];
-  if (u0 == begin || prev > u0) return;  // the share begins with its tile, or an earlier one joins it
-  int s = 0;
-  s = find_seq(p, rec[3], MT);
-  const Tile t = tile_at(p, rec[3], s, MT);
-  if (r >= t.rows) return;
-  const int h = (int)rec[4];
-  auto at = [&](int j) {  // the part that share j left of this tile
-    const int k = j == b - 1 && prev != u0 ? 1 : 0;
-    return p.part + ((size_t)j * MAX_PIECES + k) * MT * (HD + 2) + (size_t)r * (HD + 2);
-  };
-  int last = b;  // shares b - 1 .. last hold parts of the tile
-  while (last + 1 < p.grid && p.rec[(size_t)last * 8 + 5] < u1) last++;
-  float m = -INFINITY;
-  for (int j = b - 1 + lane; j <= last; j += 32) m = fmaxf(m, at(j)[0]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float mu = m == -INFINITY ? 0.0f : m;
-  float l = 0.0f, acc[N] = {};
-#pragma unroll 4
-  for (int j = b - 1; j <= last; j++) {
-    const float* x = at(j);
-    const float f = ex2(x[0] - mu);
-    l += f * x[1];
-#pragma unroll
-    for (int k = 0; k < N; k++) acc[k] += f * x[2 + 32 * k + lane];
-  }
-  const int rr = t.r0 + r;
-  T* o = static_cast<T*>(p.out) + (long long)(t.q0 + rr / p.share) * p.ld_out +
-         (long long)(h * p.share + rr % p.share) * HD;
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-  for (int k = 0; k < N; k++) o[32 * k + lane] = Elem<DT>::narrow(acc[k] * inv);
-}
-
 constexpr int CTAS_PER_SM = 2;
 
-struct Plan {
-  int mt, grid, slots;
-  size_t rec_bytes, part_bytes;
-};
-
-// Tiles of 16 rows while the batch has at most 16 (query, query head) rows a sequence and KV head on average.
-static vxg_status plan(int total, int n_seq, int heads, int kv, int hd, Plan* pl) {
-  const long long share = heads / kv;
-  pl->mt = (long long)total * share <= 16LL * n_seq ? 16 : 64;
-  const long long slots = (long long)total * share / pl->mt + n_seq;
+// The three kernels by the average number of (query, query head) rows a sequence and KV head has: up to 16 rows, tiles of
+// 16; up to 96, tiles of 64; beyond, tiles of 256 on tcgen05 (16-bit queries).
+static vxg_status plan(int total, int n_seq, int heads, int kv, int hd, int dtype, Plan* pl) {
+  const long long share = heads / kv, rows = (long long)total * share;
+  pl->mt = rows <= 16LL * n_seq ? 16 : rows <= 96LL * n_seq || dtype == VXG_DT_F32 ? 64 : 256;
+  const long long slots = rows / pl->mt + n_seq;
   if (slots > 0x3FFFFFFF) {
     set_error("%d rows of %d heads are more than one launch covers", total, heads);
     return VXG_ERR_UNSUPPORTED;
   }
   pl->slots = (int)slots;
-  pl->grid = sm_count() * CTAS_PER_SM;
+  pl->grid = sm_count() * (pl->mt == 256 ? 1 : CTAS_PER_SM);
   pl->rec_bytes = (size_t)pl->grid * 8 * sizeof(long long);
   pl->part_bytes = (size_t)pl->grid * MAX_PIECES * pl->mt * (hd + 2) * sizeof(float);
   return VXG_OK;
 }
 
-static vxg_status make_map(CUtensorMap* map, const vxg_kv_cache& c, const int8_t* base) {
-  return make_tmap_2d_u8(map, base, (uint64_t)c.n_pages * c.heads * c.page, (uint64_t)c.head_dim, (uint64_t)c.head_dim,
-                         (uint32_t)std::min(c.page, BK), (uint32_t)c.head_dim);
-}
-
 template <int HD, int DT, int MT>
 vxg_status launch(const Params& p, const Plan& pl, cudaStream_t st) {
+  auto make_map = [](CUtensorMap* map, const vxg_kv_cache& c, const int8_t* base) {
+    return make_tmap_2d_u8(map, base, (uint64_t)c.n_pages * c.heads * c.page, (uint64_t)c.head_dim, (uint64_t)c.head_dim,
+                           (uint32_t)std::min(c.page, BK), (uint32_t)c.head_dim);
+  };
   CUtensorMap mk, mv;
   vxg_status r = make_map(&mk, p.c, p.c.k);
   if (r == VXG_OK) r = make_map(&mv, p.c, p.c.v);
@@ -706,7 +471,7 @@ vxg_status launch(const Params& p, const Plan& pl, cudaStream_t st) {
   if ((r = smem_attr((const void*)attend_kernel<HD, DT, MT>, smem)) != VXG_OK) return r;
   attend_kernel<HD, DT, MT><<<pl.grid, THREADS, smem, st>>>(mk, mv, p);
   VXG_CUDA(cudaGetLastError());
-  join_kernel<HD, DT, MT><<<dim3(pl.grid - 1, MT / 4), 128, 0, st>>>(p);
+  join_kernel<HD, DT, MT, BK><<<dim3(pl.grid - 1, MT / 4), 128, 0, st>>>(p);
   note_launch(2);
   VXG_CUDA(cudaGetLastError());
   return VXG_OK;
@@ -719,10 +484,11 @@ using namespace vxg;
 
 extern "C" {
 
-size_t vxg_cache_attention_workspace_bytes(int total, int n_seq, int heads, int kv_heads, int head_dim) {
+size_t vxg_cache_attention_workspace_bytes(int total, int n_seq, int heads, int kv_heads, int head_dim, int dtype) {
   catt::Plan pl;
-  if (total <= 0 || n_seq <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || head_dim <= 0) return 0;
-  if (catt::plan(total, n_seq, heads, kv_heads, head_dim, &pl) != VXG_OK) return 0;
+  if (total <= 0 || n_seq <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || head_dim <= 0 || !dtype_known(dtype))
+    return 0;
+  if (catt::plan(total, n_seq, heads, kv_heads, head_dim, dtype, &pl) != VXG_OK) return 0;
   return pl.rec_bytes + pl.part_bytes;
 }
 
@@ -745,7 +511,7 @@ vxg_status vxg_cache_attention(const vxg_kv_cache* c, const void* q, long long l
   VXG_ARG((((uintptr_t)q | (uintptr_t)out | (uintptr_t)(ld_q * eb) | (uintptr_t)(ld_out * eb) | (uintptr_t)workspace) & 15) == 0,
           "q, out, their rows and the workspace must be 16-byte aligned");
   catt::Plan pl;
-  if ((r = catt::plan(total, n_seq, heads, c->heads, c->head_dim, &pl)) != VXG_OK) return r;
+  if ((r = catt::plan(total, n_seq, heads, c->heads, c->head_dim, dtype, &pl)) != VXG_OK) return r;
   VXG_ARG(ws_bytes >= pl.rec_bytes + pl.part_bytes, "workspace of %zu bytes, %zu needed", ws_bytes,
           pl.rec_bytes + pl.part_bytes);
   int* status = device_status();
@@ -757,12 +523,12 @@ vxg_status vxg_cache_attention(const vxg_kv_cache* c, const void* q, long long l
   p.status = status, p.n_seq = n_seq, p.max_pages = max_pages, p.total = total, p.heads = heads;
   p.share = heads / c->heads, p.window = window, p.causal = causal != 0, p.slots = pl.slots, p.grid = pl.grid;
   p.scale_log2 = scale * 1.44269504088896340736f;
-  const bool few = pl.mt == 16;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (pl.mt == 256) return catt::launch_tc(p, pl, c->head_dim, dtype, st);
   with_dtype(dtype, [&](auto tag) {
     constexpr int DT = decltype(tag)::value;
-    cudaStream_t st = (cudaStream_t)stream;
-    if (c->head_dim == 128) r = few ? catt::launch<128, DT, 16>(p, pl, st) : catt::launch<128, DT, 64>(p, pl, st);
-    else r = few ? catt::launch<64, DT, 16>(p, pl, st) : catt::launch<64, DT, 64>(p, pl, st);
+    if (c->head_dim == 128) r = pl.mt == 16 ? catt::launch<128, DT, 16>(p, pl, st) : catt::launch<128, DT, 64>(p, pl, st);
+    else r = pl.mt == 16 ? catt::launch<64, DT, 16>(p, pl, st) : catt::launch<64, DT, 64>(p, pl, st);
   });
   return r;
 }

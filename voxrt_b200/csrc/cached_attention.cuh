@@ -1,0 +1,257 @@
+// What the attention kernels over the paged cache share: tiles, the cut of all tiles' keys into equal shares, a share's
+// walk from piece to piece, the join of the pieces, and the operand conversions.
+#pragma once
+#include <cuda_runtime.h>
+
+#include "common.h"
+#include "dtype.cuh"
+#include "kv_cache.cuh"
+#include "ptx.cuh"
+#include "wait.cuh"
+
+namespace vxg {
+namespace catt {
+
+constexpr int MAX_PIECES = 2;  // partial results a CTA can leave: its first and its last
+
+struct Params {
+  vxg_kv_cache c;
+  const void* q;
+  void* out;
+  long long ld_q, ld_out;
+  const int* table;
+  const int* len;
+  const int* cu;
+  float* part;      // [grid][2][MT][HD + 2]
+  long long* rec;   // [grid][8]: begin, first unit and end of the tile it lies in, slot of the batch, KV head
+  int* status;
+  int n_seq, max_pages, total, heads, share, window, causal, slots, grid;
+  float scale_log2;
+};
+
+struct Plan {
+  int mt, grid, slots;
+  size_t rec_bytes, part_bytes;
+};
+
+// 256-row tiles on tcgen05, f16 and bf16 queries (cached_attention_tc.cu).
+vxg_status launch_tc(const Params& p, const Plan& pl, int head_dim, int dtype, cudaStream_t st);
+
+// One tile: MT rows of sequence s; `cost` units per KV head (0: no such tile, 1 where no key is visible).
+struct Tile {
+  int s, n, L, q0;       // sequence, its queries, its length, its first stacked row
+  int r0, rows;          // first (query, head) row and their number
+  int kmin, kmax;        // keys [kmin, kmax) that any of its rows sees
+  int blk0, nblk, cost;
+};
+
+__device__ __forceinline__ long long slot_base(const Params& p, int s, int MT) {
+  return (long long)__ldg(p.cu + s) * p.share / MT + s;
+}
+
+__device__ __forceinline__ int find_seq(const Params& p, long long slot, int MT) {
+  int lo = 0, hi = p.n_seq;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (slot_base(p, mid, MT) <= slot) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// The tile of a slot; s is a lower bound of its sequence and moves up to it.
+__device__ __forceinline__ Tile tile_at(const Params& p, long long slot, int& s, int MT, int BK) {
+  while (s + 1 < p.n_seq && slot_base(p, s + 1, MT) <= slot) s++;
+  Tile t;
+  t.s = s;
+  t.q0 = __ldg(p.cu + s);
+  const long long n = (long long)__ldg(p.cu + s + 1) - t.q0;
+  t.n = (int)n;
+  t.L = __ldg(p.len + s);
+  t.cost = 0;
+  t.nblk = 0;
+  const long long k = slot - slot_base(p, s, MT);
+  if (n == 0 || k < 0) return t;
+  if (n < 0 || t.q0 < 0 || t.q0 + n > p.total || t.L < 0 || t.L > (long long)p.max_pages * p.c.page) {
+    atomicCAS(p.status + 1, 0, VXG_DEV_CACHE_INDEX);
+    return t;
+  }
+  const long long r0 = k * MT, all = n * p.share;
+  if (r0 >= all) return t;
+  t.r0 = (int)r0;
+  t.rows = (int)(all - r0 < MT ? all - r0 : MT);
+  const int i0 = (int)(r0 / p.share), i1 = (int)((r0 + t.rows - 1) / p.share);
+  t.kmax = p.causal ? ::max(0, ::min(t.L, t.L - t.n + i1 + 1)) : t.L;
+  t.kmin = 0;
+  if (p.window > 0) t.kmin = (int)::max(0LL, (long long)t.L - t.n + i0 - p.window + 1);
+  t.blk0 = t.kmin / BK;
+  t.nblk = t.kmax > t.kmin ? (t.kmax + BK - 1) / BK - t.blk0 : 0;
+  t.cost = ::max(1, t.nblk);
+  return t;
+}
+
+// What a CTA works on: keys blk0 + off .. of tile t for KV head h, `left` units of its share to go (0: done).
+struct Piece {
+  Tile t;
+  long long slot, left;
+  int h, off, first;
+  __device__ __forceinline__ int take() const { return (int)::min((long long)(t.cost - off), left); }
+  // Moves on to the next piece. Ends the share where no tile is left, whatever the lengths have become meanwhile.
+  __device__ __forceinline__ void next(const Params& p, int MT, int BK) {
+    left -= take();
+    off = 0;
+    first = 0;
+    if (left > 0 && ++h == p.c.heads) {
+      h = 0;
+      int s = t.s;
+      do {
+        if (++slot >= p.slots) {
+          left = 0;
+          return;
+        }
+        t = tile_at(p, slot, s, MT, BK);
+      } while (t.cost == 0);
+    }
+  }
+};
+
+// The CTA's share of the line of all work units, as its first piece (left = 0: none): every thread of the block sums the
+// costs of a run of slots, one scan over the block, then the thread in whose run the share begins walks it again.
+template <int THREADS, int MT, int BK>
+__device__ __forceinline__ void find_share(const Params& p, Piece* first_s) {
+  constexpr int WARPS = THREADS / 32;
+  __shared__ long long warp_tot[WARPS];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int KV = p.c.heads;
+  if (tid == 0) first_s->left = 0;
+  const int per = (p.slots + THREADS - 1) / THREADS;
+  const int sl0 = ::min(p.slots, tid * per), sl1 = ::min(p.slots, sl0 + per);
+  const int first_seq = sl0 < sl1 ? find_seq(p, sl0, MT) : 0;
+  long long mine = 0;
+  {
+    int s = first_seq;
+    for (int i = sl0; i < sl1; i++) mine += tile_at(p, i, s, MT, BK).cost;
+  }
+  long long incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) warp_tot[warp] = incl;
+  __syncthreads();
+  long long before = 0, units = 0;
+#pragma unroll
+  for (int i = 0; i < WARPS; i++) {
+    if (i < warp) before += warp_tot[i];
+    units += warp_tot[i];
+  }
+  before += incl - mine;
+  units *= KV;
+  const long long parts = ::min((long long)gridDim.x, units);  // at least one unit a CTA
+  if (blockIdx.x < parts) {
+    const long long begin = units * blockIdx.x / parts, end = units * (blockIdx.x + 1) / parts;
+    if (begin >= before * KV && begin < (before + mine) * KV) {
+      long long at = before;
+      int s = first_seq;
+      for (int i = sl0; i < sl1; i++) {
+        const Tile t = tile_at(p, i, s, MT, BK);
+        if (begin < (at + t.cost) * KV) {
+          const long long in = begin - at * KV;
+          first_s->t = t;
+          first_s->slot = i;
+          first_s->h = (int)(in / t.cost);
+          first_s->off = (int)(in % t.cost);
+          first_s->left = end - begin;
+          first_s->first = 1;
+          long long* r = p.rec + blockIdx.x * 8;
+          r[0] = begin, r[1] = begin - first_s->off, r[2] = r[1] + t.cost, r[3] = i, r[4] = first_s->h, r[5] = end;
+          break;
+        }
+        at += t.cost;
+      }
+    }
+  }
+  __syncthreads();
+  if (tid == 0 && first_s->left == 0) p.rec[blockIdx.x * 8] = -1;  // more CTAs than units
+}
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Two int8 codes in bytes 0 and 2 of w -> two f16. Flipping a code's sign bit adds 128, and 0x64 above it makes the
+// f16 1024 + 128 + code, exactly.
+__device__ __forceinline__ uint32_t codes_to_f16(uint32_t w) {
+  const uint32_t biased = (w & 0x00FF00FFu) ^ 0x64806480u;
+  const uint32_t off = 0x64806480u;  // 1152, 1152
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&biased), *reinterpret_cast<const __half2*>(&off));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// the part of (a, b) that pack_f16 leaves out
+__device__ __forceinline__ uint32_t pack_rest(float a, float b, uint32_t hi) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  return pack_f16(a - f.x, b - f.y);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Joins the partial results of the tiles that span shares: block b looks at the tile in which share b begins, unless an
+// earlier share begins inside it too; a warp takes a row.
+template <int HD, int DT, int MT, int BK>
+__global__ void __launch_bounds__(128) join_kernel(const Params p) {
+  using T = typename Elem<DT>::type;
+  constexpr int N = HD / 32;
+  const int b = blockIdx.x + 1, lane = threadIdx.x & 31, r = blockIdx.y * 4 + (threadIdx.x >> 5);
+  const long long* rec = p.rec + (size_t)b * 8;
+  const long long begin = rec[0];
+  if (begin < 0) return;
+  const long long u0 = rec[1], u1 = rec[2], prev = rec[-8];
+  if (u0 == begin || prev > u0) return;  // the share begins with its tile, or an earlier one joins it
+  int s = 0;
+  s = find_seq(p, rec[3], MT);
+  const Tile t = tile_at(p, rec[3], s, MT, BK);
+  if (r >= t.rows) return;
+  const int h = (int)rec[4];
+  auto at = [&](int j) {  // the part that share j left of this tile
+    const int k = j == b - 1 && prev != u0 ? 1 : 0;
+    return p.part + ((size_t)j * MAX_PIECES + k) * MT * (HD + 2) + (size_t)r * (HD + 2);
+  };
+  int last = b;  // shares b - 1 .. last hold parts of the tile
+  while (last + 1 < p.grid && p.rec[(size_t)last * 8 + 5] < u1) last++;
+  float m = -INFINITY;
+  for (int j = b - 1 + lane; j <= last; j += 32) m = fmaxf(m, at(j)[0]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float mu = m == -INFINITY ? 0.0f : m;
+  float l = 0.0f, acc[N] = {};
+#pragma unroll 4
+  for (int j = b - 1; j <= last; j++) {
+    const float* x = at(j);
+    const float f = ex2(x[0] - mu);
+    l += f * x[1];
+#pragma unroll
+    for (int k = 0; k < N; k++) acc[k] += f * x[2 + 32 * k + lane];
+  }
+  const int rr = t.r0 + r;
+  T* o = static_cast<T*>(p.out) + (long long)(t.q0 + rr / p.share) * p.ld_out +
+         (long long)(h * p.share + rr % p.share) * HD;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+  for (int k = 0; k < N; k++) o[32 * k + lane] = Elem<DT>::narrow(acc[k] * inv);
+}
+
+}  // namespace catt
+}  // namespace vxg

@@ -45,57 +45,65 @@ def _ptr(t):
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}  # vxg_dtype
 
 
-def _need(ok, what: str):
-    if not ok:
-        raise ValueError(what)
-
-
 def _dt(t: torch.Tensor) -> int:
-    _need(t.dtype in _DTYPES, f"element type {t.dtype} is none of float16, bfloat16, float32")
-    return _DTYPES[t.dtype]
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"element type {t.dtype} is none of float16, bfloat16, float32")
+    return code
 
 
-def _rows(t: torch.Tensor, shape, what: str) -> int:
-    """Row stride in elements of a 2-D operand whose rows are contiguous."""
-    n, d = shape
-    _need(t.dim() == 2 and tuple(t.shape) == (n, d), f"{what} has shape {tuple(t.shape)}, not {(n, d)}")
-    _need(d == 1 or t.stride(1) == 1, f"{what}'s rows must be contiguous")
+def _rows(t: torch.Tensor, n: int, d: int, what: str) -> int:
+    """Row stride in elements of an [n, d] operand whose rows are contiguous."""
+    if t.shape != (n, d):
+        raise ValueError(f"{what} has shape {tuple(t.shape)}, not {(n, d)}")
+    if t.is_contiguous():
+        return d
+    if d > 1 and t.stride(1) != 1:
+        raise ValueError(f"{what}'s rows must be contiguous")
     ld = t.stride(0) if n > 1 else d
-    _need(ld >= d, f"{what}'s row stride {ld} is below its width {d}")
+    if ld < d:
+        raise ValueError(f"{what}'s row stride {ld} is below its width {d}")
     return ld
 
 
-def _on(dev: torch.device, stream, *tensors):
-    """Every operand on one GPU, and a stream of that GPU."""
-    _need(dev.type == "cuda", "operands must be CUDA tensors")
+def _gpu(stream, *tensors) -> int:
+    """The index of the one GPU that every operand (None left out) and the stream are on."""
+    idx = tensors[0].get_device()
+    if idx < 0:
+        raise ValueError("operands must be CUDA tensors")
     for t in tensors:
-        _need(t is None or t.device == dev, f"operands on {dev} and {t.device if t is not None else None}")
-    _need(stream is None or stream.device == dev, f"the stream is not {dev}'s")
+        if t is not None and t.get_device() != idx:
+            raise ValueError(f"operands on {tensors[0].device} and {t.device}")
+    if stream is not None and stream.device.index != idx:
+        raise ValueError(f"the stream is not {tensors[0].device}'s")
+    return idx
 
 
-def _empty(shape, dtype, dev, stream):
-    """Memory for an output: the allocator has to know the stream that writes it."""
+def _like(t: torch.Tensor, shape, dtype, stream) -> torch.Tensor:
+    """Memory for an output on t's device: the allocator has to know the stream that writes it."""
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=dev)
+        return t.new_empty(shape, dtype=dtype)
     with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=dev)
+        return t.new_empty(shape, dtype=dtype)
 
 
-def _call(fn, dev: torch.device, stream, used, *args):
-    """A C entry on the operands' device. On a stream other than the current one, the allocator is told which operands
-    are in use there, so that memory freed by the caller meanwhile is not handed out early."""
+def _call(fn, idx: int, stream, used, *args):
+    """A C entry on GPU `idx`. On a stream other than the current one, the allocator is told which operands are in use
+    there, so that memory freed by the caller meanwhile is not handed out early."""
     if stream is None:
-        raw = torch._C._cuda_getCurrentRawStream(dev.index)
+        raw = torch._C._cuda_getCurrentRawStream(idx)
     else:
         raw = stream.cuda_stream
         for t in used:
             if t is not None:
                 t.record_stream(stream)
-    if torch.cuda.current_device() == dev.index:
-        check(fn(*args, raw))
+    if torch.cuda.current_device() == idx:
+        status = fn(*args, raw)
     else:
-        with torch.cuda.device(dev):
-            check(fn(*args, raw))
+        with torch.cuda.device(idx):
+            status = fn(*args, raw)
+    if status:
+        check(status)
 
 
 def _addr(t):
@@ -224,40 +232,46 @@ def quantize(x: torch.Tensor, group: int = GROUP, stream=None) -> QuantAct:
         s = torch.empty((n, inp // group), dtype=torch.float32, device=x.device)
         check(lib().vxg_quantize_rows(_ptr(x), n, inp, group, _ptr(q), _ptr(s), _stream_ptr(stream)))
         return QuantAct(q, s, group)
-    _on(x.device, stream, x)
-    _need(x.dim() == 2 and x.shape[1] > 0 and group > 0, "quantize takes rows")
+    idx = _gpu(stream, x)
+    if x.dim() != 2 or x.shape[1] == 0 or group <= 0:
+        raise ValueError("quantize takes rows")
     n, d = x.shape
-    ld = _rows(x, (n, d), "x")
-    q = _empty((n, d), torch.int8, x.device, stream)
-    s = _empty((n, d // group), torch.float32, x.device, stream)
-    _call(lib().vxg_quantize_tokens, x.device, stream, (x,), _addr(x), ld, _dt(x), n, d, group, _addr(q), _addr(s))
+    dt, ld = _dt(x), _rows(x, n, d, "x")
+    q = _like(x, (n, d), torch.int8, stream)
+    s = _like(x, (n, d // group), torch.float32, stream)
+    _call(lib().vxg_quantize_tokens, idx, stream, (x,), x.data_ptr(), ld, dt, n, d, group, q.data_ptr(), s.data_ptr())
     return QuantAct(q, s, group)
 
 
 def dequantize(x: QuantAct, dtype: torch.dtype = torch.float32, stream=None) -> torch.Tensor:
     """The values that the codes stand for, q * scale, rounded once to `dtype`."""
-    dev = x.x.device
-    _on(dev, stream, x.x, x.scales)
-    _need(dtype in _DTYPES, f"element type {dtype} is none of float16, bfloat16, float32")
-    out = _empty((x.n, x.inp), dtype, dev, stream)
-    _call(lib().vxg_dequantize_rows, dev, stream, (x.x, x.scales), _addr(x.x), _addr(x.scales), x.n, x.inp, x.group,
-          _DTYPES[dtype], _addr(out))
+    q, s = x.x, x.scales
+    idx = _gpu(stream, q, s)
+    if dtype not in _DTYPES:
+        raise ValueError(f"element type {dtype} is none of float16, bfloat16, float32")
+    out = _like(q, q.shape, dtype, stream)
+    _call(lib().vxg_dequantize_rows, idx, stream, (q, s), q.data_ptr(), s.data_ptr(), x.n, x.inp, x.group,
+          _DTYPES[dtype], out.data_ptr())
     return out
 
 
-def _rms(x, gamma, eps, v, vs, x_res, y, group, q, s, stream):
-    dev = x.device
-    _on(dev, stream, gamma, v, x_res, y)
-    _need(x.dim() == 2, "x must be [n, d]")
-    shape, dt = tuple(x.shape), _dt(x)
-    _need(gamma.dtype == torch.float32 and gamma.is_contiguous() and gamma.numel() == shape[1],
-          "gamma must be d contiguous float32 values")
-    ld = []
-    for t, what in ((x, "x"), (v, "v"), (x_res, "x_res"), (y, "y")):
-        _need(t is None or t.dtype == x.dtype, f"{what} must have x's element type")
-        ld.append(0 if t is None else _rows(t, shape, what))
-    _call(lib().vxg_rms_quant, dev, stream, (x, gamma, v, x_res, y), _addr(x), ld[0], _addr(v), ld[1], float(vs), dt,
-          shape[0], shape[1], _addr(gamma), float(eps), _addr(x_res), ld[2], _addr(y), ld[3], group, _addr(q), _addr(s))
+def _rms(x, n, d, gamma, eps, v, vs, x_res, y, group, q, s, stream):
+    idx = _gpu(stream, x, gamma, v, x_res, y)
+    dt = _dt(x)
+    if gamma.dtype != torch.float32 or not gamma.is_contiguous() or gamma.numel() != d:
+        raise ValueError("gamma must be d contiguous float32 values")
+    ld_v = ld_r = ld_y = 0
+    if v is not None:
+        ld_v = _rows(v, n, d, "v")
+    if x_res is not None:
+        ld_r = _rows(x_res, n, d, "x_res")
+    if y is not None:
+        ld_y = _rows(y, n, d, "y")
+    for t in (v, x_res, y):
+        if t is not None and t.dtype != x.dtype:
+            raise ValueError("v, x_res and y must have x's element type")
+    _call(lib().vxg_rms_quant, idx, stream, (x, gamma, v, x_res, y), x.data_ptr(), _rows(x, n, d, "x"), _addr(v), ld_v, vs,
+          dt, n, d, gamma.data_ptr(), eps, _addr(x_res), ld_r, _addr(y), ld_y, group, _addr(q), _addr(s))
 
 
 def rms_quant(x: torch.Tensor, gamma: torch.Tensor, group: int | None = None, eps: float = 1e-6,
@@ -266,21 +280,26 @@ def rms_quant(x: torch.Tensor, gamma: torch.Tensor, group: int | None = None, ep
     """RMSNorm -> int8 with the residual add in front, in one pass: h = x + vs * v (stored to x_res, which may be x),
     h / sqrt(mean h^2 + eps) * gamma (stored to y, unquantised, when given), then int8 per token (group None or d: for
     gemm_i8) or per `group` columns (128: for the ternary GEMMs). f32, f16 or bf16 rows of any stride; gamma f32."""
-    _need(x.dim() == 2 and x.shape[1] > 0, "x must be [n, d]")
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise ValueError("x must be [n, d]")
     n, d = x.shape
     group = d if group is None else int(group)
-    _need(group > 0 and d % group == 0, f"group {group} does not divide the row width {d}")
-    _on(x.device, stream, x)
-    q = _empty((n, d), torch.int8, x.device, stream)
-    s = _empty((n, d // group), torch.float32, x.device, stream)
-    _rms(x, gamma, eps, v, vs, x_res, y, group, q, s, stream)
+    if group <= 0 or d % group != 0:
+        raise ValueError(f"group {group} does not divide the row width {d}")
+    if x.get_device() < 0:
+        raise ValueError("operands must be CUDA tensors")
+    q = _like(x, (n, d), torch.int8, stream)
+    s = _like(x, (n, d // group), torch.float32, stream)
+    _rms(x, n, d, gamma, eps, v, vs, x_res, y, group, q, s, stream)
     return QuantAct(q, s, group)
 
 
 def rms_norm(x: torch.Tensor, gamma: torch.Tensor, out: torch.Tensor, eps: float = 1e-6, v: torch.Tensor | None = None,
              vs: float = 1.0, x_res: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """rms_quant without the quantisation (the norm in front of an output head) -> out (may be x if x_res is not)."""
-    _rms(x, gamma, eps, v, vs, x_res, out, 1, None, None, stream)
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise ValueError("x must be [n, d]")
+    _rms(x, *x.shape, gamma, eps, v, vs, x_res, out, 1, None, None, stream)
     return out
 
 
@@ -288,10 +307,12 @@ class Int8Matrix:
     """int8 weights [out, inp] with one f32 scale per output row, resident on the GPU: gemm_i8's weights."""
 
     def __init__(self, w: torch.Tensor, scales: torch.Tensor):
-        _need(w.dtype == torch.int8 and w.is_cuda and w.dim() == 2 and w.is_contiguous(), "weights must be [out, inp] int8")
+        if w.dtype != torch.int8 or w.get_device() < 0 or w.dim() != 2 or not w.is_contiguous():
+            raise ValueError("weights must be a contiguous int8 CUDA tensor [out, inp]")
         self.out, self.inp = w.shape
-        _need(scales.dtype == torch.float32 and scales.device == w.device and scales.is_contiguous() and
-              scales.numel() == self.out, "one float32 scale per output row, on the weights' device")
+        if (scales.dtype != torch.float32 or scales.get_device() != w.get_device() or not scales.is_contiguous() or
+                scales.numel() != self.out):
+            raise ValueError("one float32 scale per output row, on the weights' device")
         self.w, self.scales = w, scales
 
     @classmethod
@@ -305,15 +326,16 @@ def gemm_i8(w: Int8Matrix, x: QuantAct, y: torch.Tensor, bias: torch.Tensor | No
             ep: Epilogue = Epilogue.Store, stream=None) -> torch.Tensor:
     """y[n, out] = epilogue(x w^T + bias) for int8 activations with one scale a token: exact int32 sums, then
     sum * (token scale * channel scale). y: f32, f16 or bf16 rows of any stride, read first for AddScaled."""
-    dev = w.w.device
-    _on(dev, stream, x.x, x.scales, y, bias)
-    _need(x.inp == w.inp and x.group == x.inp, f"activations of width {x.inp} and group {x.group} for weights of width "
-          f"{w.inp}: one scale a token is wanted")
-    _need(bias is None or (bias.dtype == torch.float32 and bias.is_contiguous() and bias.numel() == w.out),
-          "bias must be `out` contiguous float32 values")
-    ld = _rows(y, (x.n, w.out), "y")
-    _call(lib().vxg_gemm_i8, dev, stream, (x.x, x.scales, w.w, w.scales, y, bias), _addr(x.x), _addr(x.scales),
-          _addr(w.w), _addr(w.scales), x.n, w.out, w.inp, ep.kind, ep.scale, _addr(bias), _dt(y), _addr(y), ld)
+    wq, xq, sx = w.w, x.x, x.scales
+    idx = _gpu(stream, wq, xq, sx, y, bias)
+    n, out, inp = x.n, w.out, w.inp
+    if x.inp != inp or x.group != inp:
+        raise ValueError(f"activations of width {x.inp} and group {x.group} for weights of width {inp}: one scale a token "
+                         "is wanted")
+    if bias is not None and (bias.dtype != torch.float32 or not bias.is_contiguous() or bias.numel() != out):
+        raise ValueError("bias must be `out` contiguous float32 values")
+    _call(lib().vxg_gemm_i8, idx, stream, (xq, sx, wq, w.scales, y, bias), xq.data_ptr(), sx.data_ptr(), wq.data_ptr(),
+          w.scales.data_ptr(), n, out, inp, ep.kind, ep.scale, _addr(bias), _dt(y), y.data_ptr(), _rows(y, n, out, "y"))
     return y
 
 
