@@ -81,7 +81,7 @@ def test_bad_cache(kw, want):
 
 @pytest.mark.parametrize("kw,want", [
     (dict(table=None), ARG), (dict(cu=None), ARG), (dict(total=-1), ARG), (dict(n_seq=-1), ARG), (dict(width=0), ARG),
-    (dict(dt=7), ARG), (dict(total=0), OK), (dict(n_seq=0), OK), (dict(n_seq=0, table=None, cu=None), OK)])
+    (dict(dt=7), ARG), (dict(width=1 << 27), UNSUP), (dict(total=0), OK), (dict(n_seq=0), OK), (dict(n_seq=0, table=None, cu=None), OK)])
 def test_bad_batch(kw, want):
     c = _cache()
     assert _write(c, **kw) == want and _attend(c, **kw) == want and _read(c, **kw) == want

@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(THREADS, 2)
   __shared__ Piece piece_s;  // few rows: the consumers' next one
   __shared__ int fail;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int KV = p.c.heads, P = p.c.page;
+  const int KV = p.c.heads, PL = p.page_log2, P = 1 << PL;  // pages are powers of two
 
   if (tid == 0) {
     for (int i = 0; i < Lay::STAGES; i++) {
@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(THREADS, 2)
         int pid = -1;
         float ks = 0.0f, vs = 0.0f;
         for (int b = t.blk0 + off; b < t.blk0 + off + take; b++, it++) {
-          const int pg0 = b * BK / P, npg = BK > P ? BK / P : 1;
+          const int pg0 = (b * BK) >> PL, npg = BK > P ? BK >> PL : 1;
           if (have < 0 || pg0 + npg > have + 32) {
             have = pg0;
             const int pg = pg0 + lane;
@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(THREADS, 2)
             ok = false;
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          const int src = pg0 - have + (lane & 3) * 16 / P;  // page of the block's 16-key piece lane & 3
+          const int src = pg0 - have + ((lane & 3) * 16 >> PL);  // page of the block's 16-key piece lane & 3
           const float a = __shfl_sync(0xffffffffu, ks, src & 31), v = __shfl_sync(0xffffffffu, vs, src & 31);
           if (lane < 8) scales_s[st * 8 + lane] = lane < 4 ? a : v;
           const unsigned valid = __ballot_sync(0xffffffffu, pid >= 0);
@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(THREADS, 2)
           __syncwarp();
           const int mypage = lane - (pg0 - have);
           if (mypage >= 0 && mypage < npg && pid >= 0) {
-            const int row = (int)(((long long)pid * KV + h) * P) + (P > BK ? b * BK % P : 0);
+            const int row = (int)(((long long)pid * KV + h) * P) + ((b * BK) & (P - 1));
             uint8_t* dst = smem + st * Lay::STAGE + mypage * box * HD;
             tma_load_2d(dst, &map_k, 0, row, full + st);
             tma_load_2d(dst + Lay::TILE, &map_v, 0, row, full + st);
@@ -458,13 +458,9 @@ static vxg_status plan(int total, int n_seq, int heads, int kv, int hd, int dtyp
 
 template <int HD, int DT, int MT>
 vxg_status launch(const Params& p, const Plan& pl, cudaStream_t st) {
-  auto make_map = [](CUtensorMap* map, const vxg_kv_cache& c, const int8_t* base) {
-    return make_tmap_2d_u8(map, base, (uint64_t)c.n_pages * c.heads * c.page, (uint64_t)c.head_dim, (uint64_t)c.head_dim,
-                           (uint32_t)std::min(c.page, BK), (uint32_t)c.head_dim);
-  };
   CUtensorMap mk, mv;
-  vxg_status r = make_map(&mk, p.c, p.c.k);
-  if (r == VXG_OK) r = make_map(&mv, p.c, p.c.v);
+  vxg_status r = cache_map(&mk, p.c, p.c.k, BK);
+  if (r == VXG_OK) r = cache_map(&mv, p.c, p.c.v, BK);
   if (r != VXG_OK) return r;
   constexpr int smem = (int)Layout<HD, MT>::BYTES;
   static_assert((smem + 1024) * CTAS_PER_SM <= 228 * 1024, "two blocks share an SM");
@@ -498,7 +494,7 @@ vxg_status vxg_cache_attention(const vxg_kv_cache* c, const void* q, long long l
                                void* stream) {
   clear_error();
   vxg_status r = cache_check(c);
-  if (r == VXG_OK) r = cache_batch_check(table, n_seq, max_pages, len, cu, total);
+  if (r == VXG_OK) r = cache_batch_check(c, table, n_seq, max_pages, len, cu, total);
   if (r != VXG_OK) return r;
   VXG_ARG(dtype_known(dtype), "unknown element type %d", dtype);
   VXG_ARG(heads > 0 && heads % c->heads == 0, "%d query heads for %d key / value heads", heads, c->heads);
@@ -522,6 +518,7 @@ vxg_status vxg_cache_attention(const vxg_kv_cache* c, const void* q, long long l
   p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.rec_bytes);
   p.status = status, p.n_seq = n_seq, p.max_pages = max_pages, p.total = total, p.heads = heads;
   p.share = heads / c->heads, p.window = window, p.causal = causal != 0, p.slots = pl.slots, p.grid = pl.grid;
+  for (p.page_log2 = 4; 1 << p.page_log2 < c->page;) p.page_log2++;
   p.scale_log2 = scale * 1.44269504088896340736f;
   cudaStream_t st = (cudaStream_t)stream;
   if (pl.mt == 256) return catt::launch_tc(p, pl, c->head_dim, dtype, st);

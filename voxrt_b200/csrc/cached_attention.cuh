@@ -26,6 +26,7 @@ struct Params {
   long long* rec;   // [grid][8]: begin, first unit and end of the tile it lies in, slot of the batch, KV head
   int* status;
   int n_seq, max_pages, total, heads, share, window, causal, slots, grid;
+  int page_log2;
   float scale_log2;
 };
 
@@ -36,6 +37,12 @@ struct Plan {
 
 // 256-row tiles on tcgen05, f16 and bf16 queries (cached_attention_tc.cu).
 vxg_status launch_tc(const Params& p, const Plan& pl, int head_dim, int dtype, cudaStream_t st);
+
+// Rows of codes [n_pages * heads * page][head_dim], copied in boxes of a page or `most` rows.
+inline vxg_status cache_map(CUtensorMap* map, const vxg_kv_cache& c, const int8_t* base, int most) {
+  return make_tmap_2d_u8(map, base, (uint64_t)c.n_pages * c.heads * c.page, (uint64_t)c.head_dim, (uint64_t)c.head_dim,
+                         (uint32_t)(c.page < most ? c.page : most), (uint32_t)c.head_dim);
+}
 
 // One tile: MT rows of sequence s; `cost` units per KV head (0: no such tile, 1 where no key is visible).
 struct Tile {
@@ -80,7 +87,7 @@ __device__ __forceinline__ Tile tile_at(const Params& p, long long slot, int& s,
   if (r0 >= all) return t;
   t.r0 = (int)r0;
   t.rows = (int)(all - r0 < MT ? all - r0 : MT);
-  const int i0 = (int)(r0 / p.share), i1 = (int)((r0 + t.rows - 1) / p.share);
+  const int i0 = t.r0 / p.share, i1 = (t.r0 + t.rows - 1) / p.share;
   t.kmax = p.causal ? ::max(0, ::min(t.L, t.L - t.n + i1 + 1)) : t.L;
   t.kmin = 0;
   if (p.window > 0) t.kmin = (int)::max(0LL, (long long)t.L - t.n + i0 - p.window + 1);

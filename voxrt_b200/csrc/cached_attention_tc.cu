@@ -1,8 +1,8 @@
 // Attention over the paged int8 cache for many queries: tiles of 256 (query, query head) rows on tcgen05.
 //
-// A CTA holds two halves of 128 rows. Per block of 128 keys, four warps turn the codes into f16 operands in shared memory
-// (keys as they are, values times v_scale / ref * 2^8 with ref the largest value scale of the piece, rounding 2^-11),
-// one thread issues S = Q K^T and O += P V for both halves in turn, and a warpgroup a half does the softmax: a thread
+// A CTA holds two halves of 128 rows. Per block of 128 keys, one warp brings the codes by TMA, four turn them into f16
+// operands in shared memory (keys as they are, values times v_scale / ref * 2^8 with ref the largest value scale of the
+// piece, rounding 2^-11), one thread issues S = Q K^T and O += P V for both halves in turn, and a warpgroup a half does the softmax: a thread
 // owns a row, reads its 128 scores from TMEM twice (maximum, then exponentials) and writes the probabilities back over
 // them as f16, which is the second product's operand. While one half is in its softmax the tensor cores work for the
 // other. The row's reference maximum only moves when a score exceeds it by more than 8 (in powers of two): probabilities
@@ -20,9 +20,11 @@ namespace catt {
 namespace tc {
 
 constexpr int MT = 256, BK = 128;
-constexpr int SOFT_WARPS = 8, CONV_WARPS = 4, MMA_WARP = SOFT_WARPS + CONV_WARPS;
-constexpr int THREADS = (MMA_WARP + 1) * 32;
-constexpr int RING = 4;  // blocks (scales) and pieces (ref) that the converting warps can be ahead, and one more
+constexpr int SOFT_WARPS = 8, CONV_WARPS = 4, MMA_WARP = SOFT_WARPS + CONV_WARPS, LOAD_WARP = MMA_WARP + 1;
+constexpr int THREADS = (LOAD_WARP + 1) * 32;
+// Blocks' scales and pieces' refs in flight: the loading warp fills block j only after block j - 1 has found a free operand
+// stage, so after the scores of j - 3 and the softmax of j - 4; half of these would do.
+constexpr int RING = 8;
 
 template <int HD>
 struct Layout {
@@ -31,10 +33,13 @@ struct Layout {
   static constexpr uint32_t Q = 0;                        // [2]
   static constexpr uint32_t K = Q + 2 * OPER;             // [2]
   static constexpr uint32_t V = K + 2 * OPER;             // [2]
-  static constexpr uint32_t KS = V + 2 * OPER;            // [RING][8] f32
-  static constexpr uint32_t REF = KS + RING * 32;         // [RING] f32
+  static constexpr uint32_t RAW = 128 * HD;               // a block's codes
+  static constexpr uint32_t RK = V + 2 * OPER, RV = RK + RAW;
+  static constexpr uint32_t KS = RV + RAW;                // [RING][8] f32: key scales of the block's 16-key pieces
+  static constexpr uint32_t VF = KS + RING * 32;          // [RING][8] f32: their value scales / ref * 2^8
+  static constexpr uint32_t REF = VF + RING * 32;         // [RING] f32
   static constexpr uint32_t BARS = REF + RING * 4;
-  static constexpr uint32_t BYTES = BARS + 20 * 8 + 1024;
+  static constexpr uint32_t BYTES = BARS + 21 * 8 + 1024;
   static_assert(BYTES <= 232448, "shared memory budget");
 };
 
@@ -65,21 +70,24 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 template <int HD, int DT>
-__global__ void __launch_bounds__(THREADS, 1) attend_tc_kernel(const Params p) {
+__global__ void __launch_bounds__(THREADS, 1)
+    attend_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Params p) {
   using Lay = Layout<HD>;
   using T = typename Elem<DT>::type;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   float* ks_s = reinterpret_cast<float*>(smem + Lay::KS);
+  float* vf_s = reinterpret_cast<float*>(smem + Lay::VF);
   float* ref_s = reinterpret_cast<float*>(smem + Lay::REF);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Lay::BARS);
   uint64_t *kfull = bars, *kempty = bars + 2, *vfull = bars + 4, *vempty = bars + 6;  // by stage
   uint64_t *qfull = bars + 8, *sfull = bars + 10, *pfull = bars + 12, *ofull = bars + 14;  // by half
   uint64_t* drain = bars + 16;
+  uint64_t *rkfull = bars + 17, *rkempty = bars + 18, *rvfull = bars + 19, *rvempty = bars + 20;
   __shared__ Piece first_s;
   __shared__ uint32_t holder;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int KV = p.c.heads, P = p.c.page;
+  const int KV = p.c.heads, PL = p.page_log2;  // pages are powers of two
 
   if (tid == 0) {
     for (int i = 0; i < 2; i++) {
@@ -93,6 +101,10 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tc_kernel(const Params p) {
       mbar_init(ofull + i, 1);
     }
     mbar_init(drain, 1);
+    mbar_init(rkfull, 1);
+    mbar_init(rkempty, CONV_WARPS);
+    mbar_init(rvfull, 1);
+    mbar_init(rvempty, CONV_WARPS);
     fence_mbar_init();
   }
   if (warp == MMA_WARP) {
@@ -106,63 +118,88 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tc_kernel(const Params p) {
   const uint32_t tmem = holder;
   const Piece first = first_s;
 
-  if (warp >= SOFT_WARPS && warp < MMA_WARP) {
-    // ---------------------------------------------------------------------------------------- codes -> operands
-    // Pass i of a block covers its keys 16 i .. 16 i + 15, which lie in one page: warp v takes four of them, eight lanes
-    // (16 codes each) a key.
-    constexpr int LPK = HD / 16, KPW = 32 / LPK;          // lanes a key, keys a warp and pass
-    constexpr int PASSES = BK / (CONV_WARPS * KPW);        // 8 for 128 columns, 4 for 64
+  if (warp == LOAD_WARP) {
+    // ------------------------------------------------------------------------------------------------- loader
+    // Lane l holds the page and scales of the block's 16-key piece l; a page's first piece brings it.
     constexpr int CHUNKS = BK / 16;
-    const int cw = warp - SOFT_WARPS, kk = cw * KPW + lane / LPK, e0 = lane % LPK * 16;
-    uint4 kr[PASSES], vr[PASSES];
-    int pid = -1;           // page of the block's 16-key piece `lane` (lanes 0 .. 7)
-    float ksl = 0.0f, vsl = 0.0f;
-    float ref = 0.0f, vf_l = 0.0f;
+    const int ppp = 1 << (PL - 4), box = ::min(128, 1 << PL);  // pieces of a page, rows of a copy
     bool ok = true;
-    auto pages = [&](const Blocks& x) {
-      pid = -1, ksl = 0.0f, vsl = 0.0f;
+    float ref = 0.0f;
+    int it = 0;
+    for (Blocks x(p, first); !x.done() && ok; x.next(p), it++) {
       const Tile& t = x.w.t;
-      const long long key = (long long)(t.blk0 + x.w.off + x.b) * BK + 16 * lane;
-      const long long pg = key / P;
-      if (lane < CHUNKS && pg * P < t.kmax && (pg + 1) * P > t.kmin) {
-        pid = __ldg(p.table + (size_t)t.s * p.max_pages + pg);
-        if (pid < 0 || pid >= p.c.n_pages) {
+      const int key0 = (t.blk0 + x.w.off + x.b) * BK, h = x.w.h;
+      int pid = -1;
+      float ks = 0.0f, vs = 0.0f;
+      auto page_id = [&](int pg) {
+        int id = __ldg(p.table + (size_t)t.s * p.max_pages + pg);
+        if (id < 0 || id >= p.c.n_pages) {
           atomicCAS(p.status + 1, 0, VXG_DEV_CACHE_INDEX);
-          pid = -1;
-        } else {
-          ksl = __ldg(p.c.k_scales + (size_t)pid * KV + x.w.h);
-          vsl = __ldg(p.c.v_scales + (size_t)pid * KV + x.w.h);
+          id = -1;
+        }
+        return id;
+      };
+      if (x.b == 0) {  // the piece's largest value scale
+        const int k0 = ::max(key0, t.kmin), k1 = ::min(key0 + x.nb * BK, t.kmax);
+        ref = 0.0f;
+        for (int pg = (k0 >> PL) + lane; pg << PL < k1; pg += 32) {
+          const int id = page_id(pg);
+          if (id >= 0) ref = fmaxf(ref, __ldg(p.c.v_scales + (size_t)id * KV + h));
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, o));
+      }
+      const int pg = (key0 + 16 * lane) >> PL;
+      if (lane < CHUNKS && pg << PL < t.kmax && (pg + 1) << PL > t.kmin) {  // a page that some row sees
+        pid = page_id(pg);
+        if (pid >= 0) {
+          ks = __ldg(p.c.k_scales + (size_t)pid * KV + h);
+          vs = __ldg(p.c.v_scales + (size_t)pid * KV + h);
         }
       }
-    };
-    auto load = [&](const Blocks& x, const int8_t* codes, uint4 (&r)[PASSES]) {
-      const long long key0 = (long long)(x.w.t.blk0 + x.w.off + x.b) * BK;
-#pragma unroll
-      for (int i = 0; i < PASSES; i++) {
-        const int k = i * CONV_WARPS * KPW + kk;
-        const int id = __shfl_sync(0xffffffffu, pid, k / 16);
-        r[i] = make_uint4(0, 0, 0, 0);
-        if (id >= 0 && key0 + k < x.w.t.kmax)
-          r[i] = __ldg(reinterpret_cast<const uint4*>(codes + (((size_t)id * KV + x.w.h) * P + (size_t)((key0 + k) % P)) * HD + e0));
+      const bool bring = pid >= 0 && lane % ppp == 0;
+      const uint32_t bytes = (uint32_t)__popc(__ballot_sync(0xffffffffu, bring)) * box * HD;
+      const int row = (pid * KV + h) << PL;
+      if (it > 0 && !wait_phase(rkempty, (it - 1) & 1, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN)) ok = false;
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if (lane < CHUNKS) {
+        ks_s[(it % RING) * 8 + lane] = ks;
+        vf_s[(it % RING) * 8 + lane] = ref > 0.0f ? vs / ref * 256.0f : 0.0f;
       }
-    };
-    auto largest = [&](const Blocks& x) {  // the piece's largest value scale
-      const Tile& t = x.w.t;
-      const long long k0 = ::max((long long)(t.blk0 + x.w.off) * BK, (long long)t.kmin);
-      const long long k1 = ::min((long long)(t.blk0 + x.w.off + x.nb) * BK, (long long)t.kmax);
-      float m = 0.0f;
-      for (long long pg = k0 / P + lane; pg * P < k1; pg += 32) {
-        const int id = __ldg(p.table + (size_t)t.s * p.max_pages + pg);
-        if (id >= 0 && id < p.c.n_pages) m = fmaxf(m, __ldg(p.c.v_scales + (size_t)id * KV + x.w.h));
+      if (lane == 8 && x.b == 0) ref_s[x.piece % RING] = ref;
+      __syncwarp();
+      if (lane == 0) mbar_arrive_expect_tx(rkfull, bytes);
+      __syncwarp();
+      if (bring) tma_load_2d(smem + Lay::RK + lane * 16 * HD, &map_k, 0, row, rkfull);
+      if (it > 0 && !wait_phase(rvempty, (it - 1) & 1, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN)) ok = false;
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) {
+        it++;  // this block's keys are on their way
+        break;
       }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      return m;
+      if (lane == 0) mbar_arrive_expect_tx(rvfull, bytes);
+      __syncwarp();
+      if (bring) tma_load_2d(smem + Lay::RV + lane * 16 * HD, &map_v, 0, row, rvfull);
+    }
+    // every copy lands before the block may end
+    if (it > 0) {
+      wait_phase(rkfull, (it - 1) & 1, p.status, VXG_DEV_TIMEOUT_DRAIN);
+      if (ok) wait_phase(rvfull, (it - 1) & 1, p.status, VXG_DEV_TIMEOUT_DRAIN);
+    }
+  } else if (warp >= SOFT_WARPS && warp < MMA_WARP) {
+    // ---------------------------------------------------------------------------------------- codes -> operands
+    // Eight lanes (16 codes each; four for 64 columns) take a key, a warp four (eight) keys a pass, all in one 16-key piece.
+    constexpr int LPK = HD / 16, KPW = 32 / LPK, PASSES = BK / (CONV_WARPS * KPW);
+    const int kk = (warp - SOFT_WARPS) * KPW + lane / LPK, ch = lane % LPK, e0 = ch * 16;
+    const uint32_t swap = HD == 128 && e0 >= 64;
+    auto get = [&](const uint8_t* raw, int k) {  // the copies' swizzle: 128-byte rows by row % 8, 64-byte rows by row / 2 % 4
+      return *reinterpret_cast<const uint4*>(raw + k * HD + ((HD == 128 ? ch ^ (k & 7) : ch ^ ((k >> 1) & 3)) << 4));
     };
     // 16 codes -> two 16-byte chunks of the operand row; the upper half of the lanes of a key stores its odd chunk first,
     // so that the eight lanes of a store phase meet eight different chunks
     auto put = [&](uint8_t* dst, int k, uint4 x, bool scaled, __half2 f) {
-      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+      const uint32_t w[4] = {swap ? x.z : x.x, swap ? x.w : x.y, swap ? x.x : x.z, swap ? x.y : x.w};
       uint32_t h[8];
 #pragma unroll
       for (int i = 0; i < 4; i++) {
@@ -178,55 +215,47 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tc_kernel(const Params p) {
       }
       uint8_t* base = dst + (e0 / 64) * Lay::HALF;
       const uint32_t c = (uint32_t)(e0 % 64) / 8;
-      const bool odd = HD == 128 && e0 >= 64;
-      const uint4 a = make_uint4(h[0], h[1], h[2], h[3]), b = make_uint4(h[4], h[5], h[6], h[7]);
-      *reinterpret_cast<uint4*>(base + sw128_offset((uint32_t)k, c + (odd ? 1 : 0))) = odd ? b : a;
-      *reinterpret_cast<uint4*>(base + sw128_offset((uint32_t)k, c + (odd ? 0 : 1))) = odd ? a : b;
+      *reinterpret_cast<uint4*>(base + sw128_offset((uint32_t)k, c + swap)) = make_uint4(h[0], h[1], h[2], h[3]);
+      *reinterpret_cast<uint4*>(base + sw128_offset((uint32_t)k, c + 1 - swap)) = make_uint4(h[4], h[5], h[6], h[7]);
     };
-    Blocks x(p, first);
-    if (!x.done()) {
-      pages(x);
-      ref = largest(x);
-      load(x, p.c.k, kr);
-      load(x, p.c.v, vr);
-    }
-    for (int it = 0; !x.done(); it++) {
+    bool ok = true;
+    auto wait = [&](uint64_t* b, int phase) {
+      if (ok && !wait_phase(b, (uint32_t)phase & 1, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN)) ok = false;
+      ok = __all_sync(0xffffffffu, ok);
+      return ok;
+    };
+    int it = 0;
+    for (Blocks x(p, first); !x.done(); x.next(p), it++) {
       const int st = it & 1;
-      if (it >= 2 && !wait_phase(kempty + st, ((it >> 1) - 1) & 1, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN)) ok = false;
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      if (cw == 0) {
-        if (lane < 8) ks_s[(it % RING) * 8 + lane] = ksl;
-        if (lane == 8 && x.b == 0) ref_s[x.piece % RING] = ref;
-      }
-#pragma unroll
-      for (int i = 0; i < PASSES; i++)
-        put(smem + Lay::K + st * Lay::OPER, i * CONV_WARPS * KPW + kk, kr[i], false, __half2());
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(kfull + st);
-      vf_l = ref > 0.0f ? vsl / ref * 256.0f : 0.0f;
-      // the next block's page, scales and keys on their way before this block's values are written
-      Blocks nx = x;
-      nx.next(p);
-      if (!nx.done()) {
-        pages(nx);
-        if (nx.b == 0) ref = largest(nx);
-        load(nx, p.c.k, kr);
-      }
-      if (it >= 2 && !wait_phase(vempty + st, ((it >> 1) - 1) & 1, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN)) ok = false;
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-#pragma unroll
+      if (it >= 2 && !wait(kempty + st, (it >> 1) - 1)) break;
+      if (!wait(rkfull, it)) break;
+      uint8_t* dk = smem + Lay::K + st * Lay::OPER;
+#pragma unroll 2  // more would cost more in instruction fetches than it hides
       for (int i = 0; i < PASSES; i++) {
         const int k = i * CONV_WARPS * KPW + kk;
-        put(smem + Lay::V + st * Lay::OPER, k, vr[i], true, __float2half2_rn(__shfl_sync(0xffffffffu, vf_l, k / 16)));
+        put(dk, k, get(smem + Lay::RK, k), false, __half2());
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(vfull + st);
-      if (!nx.done()) load(nx, p.c.v, vr);
-      x = nx;
+      if (lane == 0) {
+        mbar_arrive(kfull + st);
+        mbar_arrive(rkempty);
+      }
+      if (it >= 2 && !wait(vempty + st, (it >> 1) - 1)) break;
+      if (!wait(rvfull, it)) break;
+      uint8_t* dv = smem + Lay::V + st * Lay::OPER;
+      const float* vf = vf_s + (it % RING) * 8;
+#pragma unroll 2
+      for (int i = 0; i < PASSES; i++) {
+        const int k = i * CONV_WARPS * KPW + kk;
+        put(dv, k, get(smem + Lay::RV, k), true, __float2half2_rn(vf[k / 16]));
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(vfull + st);
+        mbar_arrive(rvempty);
+      }
     }
   } else if (warp == MMA_WARP) {
     // --------------------------------------------------------------------------------------------- MMA issuer
@@ -289,7 +318,9 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tc_kernel(const Params p) {
   } else {
     // ------------------------------------------------------------------------------------------------ softmax
     const int half = warp >> 2, r = half * 128 + (warp & 3) * 32 + lane;  // the thread's row of the tile
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    constexpr int LPR = HD / 8, RPI = 32 / LPR;  // lanes a row and rows an access where a warp moves rows as wholes
+    const int wrow = (warp & 3) * 32;            // the warp's first row of its half
+    const uint32_t lanes = (uint32_t)wrow << 16;
     const uint32_t S = tmem + lanes + half * 128, O = tmem + lanes + 256 + half * HD;
     bool ok = true;
     uint32_t it = 0, pieces = 0;
@@ -303,38 +334,46 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tc_kernel(const Params p) {
       const int klo = p.window > 0 ? (int)::max(0LL, pos - p.window + 1) : 0;
       float m = -INFINITY, l = 0.0f, unit = 0.0f;
       if (nb > 0) {
-        // ---- this row of Q: scaled by a power of two, f16, into the half's operand
-        const T* q = static_cast<const T*>(p.q) + (long long)(t.q0 + i) * p.ld_q + (long long)head * HD;
-        auto chunk = [&](int c) { return live ? reinterpret_cast<const uint4*>(q)[c] : make_uint4(0, 0, 0, 0); };
-        float top = 0.0f;
-#pragma unroll 4
-        for (int c = 0; c < HD / 8; c++) {
-          const uint4 raw = chunk(c);
-          const uint32_t x[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-          for (int k = 0; k < 4; k++) {
-            const float2 f = widen2<DT>(x[k]);
-            top = max3(top, fabsf(f.x), fabsf(f.y));
-          }
-        }
-        int ex = 14 - ((int)(__float_as_uint(top) >> 23) - 127);
-        ex = top == 0.0f || !(top <= 3.402823466e38f) ? 0 : ::min(ex, 126);
-        const float up = __int_as_float((ex + 127) << 23);
-        const float rowf = __int_as_float((127 - ex) << 23) * p.scale_log2;
+        // ---- the warp's rows of Q: each scaled by a power of two, f16, into the half's operand. LPR lanes read a row.
+        const long long qoff = live ? (long long)(t.q0 + i) * p.ld_q + (long long)head * HD : -1;
         uint8_t* qs = smem + Lay::Q + half * Lay::OPER;
-#pragma unroll 4
-        for (int c = 0; c < HD / 8; c++) {  // a second time, from L1
-          const uint4 raw = chunk(c);
-          const uint32_t x[4] = {raw.x, raw.y, raw.z, raw.w};
-          uint32_t h[4];
+        int ex = 0;  // of this thread's own row
+#pragma unroll 1
+        for (int n0 = 0; n0 < LPR; n0 += 8) {
+          uint4 raw[8];
 #pragma unroll
-          for (int k = 0; k < 4; k++) {
-            const float2 f = widen2<DT>(x[k]);
-            h[k] = pack_f16(f.x * up, f.y * up);
+          for (int n = 0; n < 8; n++) {
+            const long long o = __shfl_sync(0xffffffffu, qoff, (n0 + n) * RPI + lane / LPR);
+            raw[n] = make_uint4(0, 0, 0, 0);
+            if (o >= 0) raw[n] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + o + lane % LPR * 8);
           }
-          *reinterpret_cast<uint4*>(qs + (c / 8) * Lay::HALF + sw128_offset((uint32_t)(r & 127), (uint32_t)(c % 8))) =
-              make_uint4(h[0], h[1], h[2], h[3]);
+#pragma unroll
+          for (int n = 0; n < 8; n++) {
+            const uint32_t x[4] = {raw[n].x, raw[n].y, raw[n].z, raw[n].w};
+            float2 f[4];
+            float top = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              f[k] = widen2<DT>(x[k]);
+              top = max3(top, fabsf(f[k].x), fabsf(f[k].y));
+            }
+#pragma unroll
+            for (int o = 1; o < LPR; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            int e = 14 - ((int)(__float_as_uint(top) >> 23) - 127);
+            e = top == 0.0f || !(top <= 3.402823466e38f) ? 0 : ::min(e, 126);
+            const int got = __shfl_sync(0xffffffffu, e, lane % RPI * LPR);
+            if (lane / RPI == n0 + n) ex = got;
+            const float up = __int_as_float((e + 127) << 23);
+            uint32_t h[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) h[k] = pack_f16(f[k].x * up, f[k].y * up);
+            const int c = lane % LPR;
+            *reinterpret_cast<uint4*>(qs + (c / 8) * Lay::HALF +
+                                      sw128_offset((uint32_t)(wrow + (n0 + n) * RPI + lane / LPR), (uint32_t)(c % 8))) =
+                make_uint4(h[0], h[1], h[2], h[3]);
+          }
         }
+        const float rowf = __int_as_float((127 - ex) << 23) * p.scale_log2;
         fence_proxy_async_smem();
         tc_fence_before();
         __syncwarp();
@@ -354,28 +393,36 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tc_kernel(const Params p) {
           if (b == 0) unit = ref_s[pieces % RING] * (1.0f / 256.0f);
           // ---- the block's maximum
           float mx = -INFINITY;
+          auto maximum = [&](auto tag) {
+            constexpr bool masked = decltype(tag)::value;
 #pragma unroll 1
-          for (int c = 0; c < BK; c += 32) {
-            uint32_t a[32];
-            tmem_ld32(S + c, a);
-            tmem_wait_ld();
-            if (!inside) {
+            for (int c = 0; c < BK; c += 64) {
+              uint32_t a[2][32];
+              tmem_ld32(S + c, a[0]);
+              tmem_ld32(S + c + 32, a[1]);
+              tmem_wait_ld();
 #pragma unroll
-              for (int j = 0; j < 32; j++)
-                if (key0 + c + j < klo || key0 + c + j >= khi) a[j] = 0xFF800000u;  // -inf
+              for (int g = 0; g < 4; g++) {
+                const uint32_t* v = a[g >> 1] + 16 * (g & 1);
+                float y[16];
+#pragma unroll
+                for (int j = 0; j < 16; j++) {
+                  y[j] = __uint_as_float(v[j]);
+                  const int key = key0 + c + 16 * g + j;
+                  if (masked && (key < klo || key >= khi)) y[j] = -INFINITY;
+                }
+                float x = max3(y[0], y[1], y[2]), z = max3(y[3], y[4], y[5]);
+                x = max3(x, y[6], y[7]), z = max3(z, y[8], y[9]);
+                x = max3(x, y[10], y[11]), z = max3(z, y[12], y[13]);
+                x = max3(x, y[14], y[15]), x = fmaxf(x, z);
+                // -inf x 0 would be NaN: a piece without a visible key has no maximum
+                const float f = rowf * ks[c / 16 + g];
+                mx = fmaxf(mx, masked && x == -INFINITY ? x : x * f);
+              }
             }
-#pragma unroll
-            for (int g = 0; g < 2; g++) {
-              float x = max3(__uint_as_float(a[16 * g]), __uint_as_float(a[16 * g + 1]), __uint_as_float(a[16 * g + 2]));
-#pragma unroll
-              for (int j = 3; j < 15; j += 2)
-                x = max3(x, __uint_as_float(a[16 * g + j]), __uint_as_float(a[16 * g + j + 1]));
-              x = fmaxf(x, __uint_as_float(a[16 * g + 15]));
-              const float f = rowf * ks[c / 16 + g];
-              // -inf x 0 would be NaN: a piece without a visible key has no maximum
-              mx = fmaxf(mx, x == -INFINITY ? x : x * f);
-            }
-          }
+          };
+          if (inside) maximum(std::false_type());
+          else maximum(std::true_type());
           // ---- move the reference when the maximum has outgrown it
           const bool grow = mx > m + 8.0f;
           if (__any_sync(0xffffffffu, grow)) {
@@ -396,28 +443,44 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tc_kernel(const Params p) {
           }
           const float mm = m == -INFINITY ? 0.0f : m - 7.0f;  // probabilities times 2^7
           // ---- probabilities over the scores: chunk c's 32 scores are read before its 16 columns are written
-          float l0 = 0.0f, l1 = 0.0f;
+          uint64_t sum = 0;  // two partial sums of the block
+          auto exponentials = [&](auto tag) {
+            constexpr bool masked = decltype(tag)::value;
+            const uint64_t mm2 = pk2(-mm, -mm);
+            uint32_t a[32];
+            tmem_ld32(S, a);
 #pragma unroll 1
-          for (int c = 0; c < BK; c += 32) {
-            uint32_t a[32], o[16];
-            tmem_ld32(S + c, a);
-            tmem_wait_ld();
-            const float f0 = rowf * ks[c / 16], f1 = rowf * ks[c / 16 + 1];
+            for (int c = 0; c < BK; c += 32) {
+              uint64_t x[16];
+              const float f0 = rowf * ks[c / 16], f1 = rowf * ks[c / 16 + 1];
+              tmem_wait_ld();
 #pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-              const float f = j < 16 ? f0 : f1;
-              float x0 = fmaf(__uint_as_float(a[j]), f, -mm), x1 = fmaf(__uint_as_float(a[j + 1]), f, -mm);
-              if (!inside) {
-                if (key0 + c + j < klo || key0 + c + j >= khi) x0 = -INFINITY;
-                if (key0 + c + j + 1 < klo || key0 + c + j + 1 >= khi) x1 = -INFINITY;
+              for (int j = 0; j < 16; j++) {
+                const float f = j < 8 ? f0 : f1;
+                x[j] = ffma2(pk2(__uint_as_float(a[2 * j]), __uint_as_float(a[2 * j + 1])), pk2(f, f), mm2);
               }
-              const float p0 = ex2(x0), p1 = ex2(x1);
-              l0 += p0;
-              l1 += p1;
-              o[j / 2] = pack_f16(p0, p1);
+              if (c + 32 < BK) tmem_ld32(S + c + 32, a);  // under this chunk's exponentials
+              uint32_t o[16];
+#pragma unroll
+              for (int j = 0; j < 16; j++) {
+                float x0, x1;
+                upk2(x[j], x0, x1);
+                if (masked) {
+                  const int key = key0 + c + 2 * j;
+                  if (key < klo || key >= khi) x0 = -INFINITY;
+                  if (key + 1 < klo || key + 1 >= khi) x1 = -INFINITY;
+                }
+                const float p0 = ex2(x0), p1 = ex2(x1);
+                sum = fadd2(sum, pk2(p0, p1));
+                o[j] = pack_f16(p0, p1);
+              }
+              tmem_st16(S + c / 2, o);
             }
-            tmem_st16(S + c / 2, o);
-          }
+          };
+          if (inside) exponentials(std::false_type());
+          else exponentials(std::true_type());
+          float l0, l1;
+          upk2(sum, l0, l1);
           l += l0 + l1;
           tmem_wait_st();
           tc_fence_before();
@@ -433,9 +496,9 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tc_kernel(const Params p) {
       // ---- the row's result, whole or for the join
       const bool whole = w.off == 0 && take == t.cost;
       float* part = p.part + ((size_t)blockIdx.x * MAX_PIECES + (w.first ? 0 : 1)) * MT * (HD + 2) + (size_t)r * (HD + 2);
-      T* out = static_cast<T*>(p.out) + (long long)(t.q0 + i) * p.ld_out + (long long)head * HD;
       const float inv = l == 0.0f ? 0.0f : unit / l;
       if (live && !whole) part[0] = m - 7.0f, part[1] = l;
+      uint8_t* os = smem + Lay::Q + half * Lay::OPER;  // the half's products are done with Q
 #pragma unroll 1
       for (int c = 0; c < HD; c += 32) {
         uint32_t a[32];
@@ -446,19 +509,36 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tc_kernel(const Params p) {
 #pragma unroll
           for (int j = 0; j < 32; j++) a[j] = 0;
         }
-        if (live && whole) {
+        if (whole) {
 #pragma unroll
           for (int j = 0; j < 32; j += 8) {
-            float v[8];
+            uint32_t h[4];
 #pragma unroll
-            for (int k = 0; k < 8; k++) v[k] = l == 0.0f ? 0.0f : __uint_as_float(a[j + k]) * inv;
-            store8<DT>(out + c + j, v);
+            for (int k = 0; k < 4; k++) {
+              const float v0 = __uint_as_float(a[j + 2 * k]) * inv, v1 = __uint_as_float(a[j + 2 * k + 1]) * inv;
+              h[k] = narrow2<DT>(l == 0.0f ? 0.0f : v0, l == 0.0f ? 0.0f : v1);
+            }
+            *reinterpret_cast<uint4*>(os + (c / 64) * Lay::HALF +
+                                      sw128_offset((uint32_t)(wrow + lane), (uint32_t)((c % 64 + j) / 8))) =
+                make_uint4(h[0], h[1], h[2], h[3]);
           }
         } else if (live) {
 #pragma unroll
           for (int j = 0; j < 32; j += 2)
             *reinterpret_cast<float2*>(part + 2 + c + j) =
                 make_float2(__uint_as_float(a[j]) * unit, __uint_as_float(a[j + 1]) * unit);
+        }
+        __syncwarp();
+      }
+      if (whole) {
+        const long long ooff = live ? (long long)(t.q0 + i) * p.ld_out + (long long)head * HD : -1;
+#pragma unroll 4
+        for (int n = 0; n < LPR; n++) {
+          const int row = n * RPI + lane / LPR, c = lane % LPR;
+          const long long o = __shfl_sync(0xffffffffu, ooff, row);
+          const uint4 v = *reinterpret_cast<const uint4*>(os + (c / 8) * Lay::HALF +
+                                                          sw128_offset((uint32_t)(wrow + row), (uint32_t)(c % 8)));
+          if (o >= 0) *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + o + c * 8) = v;
         }
         __syncwarp();
       }
@@ -476,9 +556,12 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tc_kernel(const Params p) {
 template <int HD, int DT>
 vxg_status launch(const Params& p, const Plan& pl, cudaStream_t st) {
   constexpr int smem = (int)Layout<HD>::BYTES;
-  const vxg_status r = smem_attr((const void*)attend_tc_kernel<HD, DT>, smem);
+  CUtensorMap mk, mv;
+  vxg_status r = smem_attr((const void*)attend_tc_kernel<HD, DT>, smem);
+  if (r == VXG_OK) r = cache_map(&mk, p.c, p.c.k, 128);
+  if (r == VXG_OK) r = cache_map(&mv, p.c, p.c.v, 128);
   if (r != VXG_OK) return r;
-  attend_tc_kernel<HD, DT><<<pl.grid, THREADS, smem, st>>>(p);
+  attend_tc_kernel<HD, DT><<<pl.grid, THREADS, smem, st>>>(mk, mv, p);
   VXG_CUDA(cudaGetLastError());
   join_kernel<HD, DT, MT, BK><<<dim3(pl.grid - 1, MT / 4), 128, 0, st>>>(p);
   note_launch(2);

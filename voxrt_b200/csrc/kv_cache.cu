@@ -199,10 +199,15 @@ vxg_status cache_check(const vxg_kv_cache* c) {
   return VXG_OK;
 }
 
-vxg_status cache_batch_check(const int* table, int n_seq, int max_pages, const int* a, const int* cu, int total) {
+vxg_status cache_batch_check(const vxg_kv_cache* c, const int* table, int n_seq, int max_pages, const int* a,
+                             const int* cu, int total) {
   VXG_ARG(n_seq >= 0 && max_pages >= 0 && total >= 0, "bad batch: %d sequences of %d pages, %d rows", n_seq, max_pages,
           total);
   VXG_ARG(n_seq == 0 || total == 0 || (table && a && cu && max_pages > 0), "NULL page table, lengths or offsets");
+  if ((long long)max_pages * c->page > 0x7FFFFF00LL) {
+    set_error("sequences of %d pages of %d tokens not supported", max_pages, c->page);
+    return VXG_ERR_UNSUPPORTED;
+  }
   return VXG_OK;
 }
 
@@ -217,7 +222,7 @@ vxg_status vxg_cache_write(const vxg_kv_cache* c, const void* k, long long ld_k,
                            void* stream) {
   clear_error();
   vxg_status r = cache_check(c);
-  if (r == VXG_OK) r = cache_batch_check(table, n_seq, max_pages, start, cu, total);
+  if (r == VXG_OK) r = cache_batch_check(c, table, n_seq, max_pages, start, cu, total);
   if (r != VXG_OK) return r;
   VXG_ARG(dtype_known(dtype), "unknown element type %d", dtype);
   if (total == 0 || n_seq == 0) return VXG_OK;
@@ -249,7 +254,7 @@ vxg_status vxg_cache_read(const vxg_kv_cache* c, const int* table, int n_seq, in
                           const int* cu, int total, int dtype, void* k, void* v, void* stream) {
   clear_error();
   vxg_status r = cache_check(c);
-  if (r == VXG_OK) r = cache_batch_check(table, n_seq, max_pages, start, cu, total);
+  if (r == VXG_OK) r = cache_batch_check(c, table, n_seq, max_pages, start, cu, total);
   if (r != VXG_OK) return r;
   VXG_ARG(dtype_known(dtype), "unknown element type %d", dtype);
   if (total == 0 || n_seq == 0) return VXG_OK;
