@@ -259,62 +259,77 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   } else if (warp == MMA_WARP) {
     // --------------------------------------------------------------------------------------------- MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t QK = idesc_f16(128, BK, false), PV = idesc_f16(128, HD, true);
-      bool ok = true;
-      uint32_t nq = 0, np = 0;  // pieces begun, probabilities consumed (per half)
-      int it = 0;
-      auto wait = [&](uint64_t* b, uint32_t phase) {
-        if (ok && !wait_phase(b, phase & 1, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN)) ok = false;
-        if (ok) tc_fence_after();
-        return ok;
-      };
-      auto scores = [&](int half, int st) {
-        const uint32_t q = smem_u32(smem + Lay::Q + half * Lay::OPER), k = smem_u32(smem + Lay::K + st * Lay::OPER);
+    // The whole warp walks and waits, so that the operand descriptors stay in uniform registers, and one lane issues.
+    // With one lane doing all of it, the descriptors' arithmetic took longer than the products.
+    constexpr uint32_t QK = idesc_f16(128, BK, false), PV = idesc_f16(128, HD, true);
+    const bool leader = elect_one();
+    // descriptor = fixed upper word, lower word = address / 16 and the offset between 64-column halves
+    const uint64_t desc_k = umma_desc_sw128(smem_u32(smem)), desc_mn = umma_desc_sw128_mn(smem_u32(smem), Lay::HALF);
+    bool ok = true;
+    uint32_t nq = 0, np = 0;  // pieces begun, probabilities consumed (per half)
+    int it = 0;
+    auto wait = [&](uint64_t* b, uint32_t phase) {
+      if (ok && !wait_phase(b, phase & 1, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN)) ok = false;
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok) tc_fence_after();
+      return ok;
+    };
+    auto scores = [&](int half, int st) {
+      const uint64_t q = desc_k + (Lay::Q + half * Lay::OPER) / 16, k = desc_k + (Lay::K + st * Lay::OPER) / 16;
+      if (leader) {
 #pragma unroll
         for (int c = 0; c < HD / 64; c++)
 #pragma unroll
           for (int j = 0; j < 4; j++)
-            mma_f16_ss(tmem + half * 128, umma_desc_sw128(q + c * Lay::HALF) + 2 * j, umma_desc_sw128(k + c * Lay::HALF) + 2 * j,
-                       QK, (c | j) != 0 ? 1u : 0u);
+            mma_f16_ss(tmem + half * 128, q + c * (Lay::HALF / 16) + 2 * j, k + c * (Lay::HALF / 16) + 2 * j, QK,
+                       (c | j) != 0 ? 1u : 0u);
         mma_commit(sfull + half);
-      };
-      auto values = [&](int half, int st, bool fresh) {
-        const uint32_t v = smem_u32(smem + Lay::V + st * Lay::OPER);
+      }
+      __syncwarp();
+    };
+    auto values = [&](int half, int st, bool fresh, bool last) {
+      const uint64_t v = desc_mn + (Lay::V + st * Lay::OPER) / 16;
+      if (leader) {
 #pragma unroll
         for (int j = 0; j < BK / 16; j++)
-          mma_f16_ts(tmem + 256 + half * HD, tmem + half * 128 + 8 * j, umma_desc_sw128_mn(v + j * 2048, Lay::HALF), PV,
-                     fresh && j == 0 ? 0u : 1u);
-      };
-      for (Blocks x(p, first); !x.done() && ok;) {
-        for (int half = 0; half < 2 && ok; half++) {
-          if (!wait(qfull + half, nq)) break;
-          if (half == 0 && !wait(kfull + (it & 1), it >> 1)) break;
-          scores(half, it & 1);
-        }
-        if (!ok) break;
-        mma_commit(kempty + (it & 1));
-        nq++;
-        const int nb = x.nb;
-        for (int b = 0; b < nb && ok; b++, it++, np++) {
-          const bool more = b + 1 < nb;
-          if (!wait(vfull + (it & 1), it >> 1)) break;
-          for (int half = 0; half < 2 && ok; half++) {
-            if (!wait(pfull + half, np)) break;
-            values(half, it & 1, b == 0);
-            if (!more) mma_commit(ofull + half);
-            if (more && half == 0 && !wait(kfull + ((it + 1) & 1), (it + 1) >> 1)) break;
-            if (more) scores(half, (it + 1) & 1);
-          }
-          if (!ok) break;
-          mma_commit(vempty + (it & 1));
-          if (more) mma_commit(kempty + ((it + 1) & 1));
-          x.next(p);
-        }
+          mma_f16_ts(tmem + 256 + half * HD, tmem + half * 128 + 8 * j, v + j * 128, PV, fresh && j == 0 ? 0u : 1u);
+        if (last) mma_commit(ofull + half);
       }
-      mma_commit(drain);  // nothing is in flight when the block ends
-      wait_phase(drain, 0, p.status, VXG_DEV_TIMEOUT_DRAIN);
+      __syncwarp();
+    };
+    auto commit = [&](uint64_t* b) {
+      if (leader) mma_commit(b);
+      __syncwarp();
+    };
+    for (Blocks x(p, first); !x.done() && ok;) {
+      if (!wait(qfull, nq) || !wait(kfull + (it & 1), it >> 1)) break;
+      scores(0, it & 1);
+      if (!wait(qfull + 1, nq)) break;
+      scores(1, it & 1);
+      commit(kempty + (it & 1));
+      nq++;
+      const int nb = x.nb;
+      for (int b = 0; b < nb; b++, it++, np++) {
+        const bool more = b + 1 < nb;
+        const int st = it & 1, sn = st ^ 1;
+        if (!wait(vfull + st, it >> 1) || !wait(pfull, np)) break;
+        values(0, st, b == 0, !more);
+        if (more) {
+          if (!wait(kfull + sn, (it + 1) >> 1)) break;
+          scores(0, sn);
+        }
+        if (!wait(pfull + 1, np)) break;
+        values(1, st, b == 0, !more);
+        commit(vempty + st);
+        if (more) {
+          scores(1, sn);
+          commit(kempty + sn);
+        }
+        x.next(p);
+      }
     }
+    commit(drain);  // nothing is in flight when the block ends
+    wait_phase(drain, 0, p.status, VXG_DEV_TIMEOUT_DRAIN);
   } else {
     // ------------------------------------------------------------------------------------------------ softmax
     const int half = warp >> 2, r = half * 128 + (warp & 3) * 32 + lane;  // the thread's row of the tile
