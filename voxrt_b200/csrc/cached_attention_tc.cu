@@ -458,7 +458,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           const float mm = m == -INFINITY ? 0.0f : m - 7.0f;  // probabilities times 2^7
           // ---- probabilities over the scores: chunk c's 32 scores are read before its 16 columns are written
-          uint64_t sum = 0;  // two partial sums of the block
+          uint64_t sum[4] = {0, 0, 0, 0};  // eight partial sums of the block
           auto exponentials = [&](auto tag) {
             constexpr bool masked = decltype(tag)::value;
             const uint64_t mm2 = pk2(-mm, -mm);
@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                   if (key + 1 < klo || key + 1 >= khi) x1 = -INFINITY;
                 }
                 const float p0 = ex2(x0), p1 = ex2(x1);
-                sum = fadd2(sum, pk2(p0, p1));
+                sum[j & 3] = fadd2(sum[j & 3], pk2(p0, p1));
                 o[j] = pack_f16(p0, p1);
               }
               tmem_st16(S + c / 2, o);
@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (inside) exponentials(std::false_type());
           else exponentials(std::true_type());
           float l0, l1;
-          upk2(sum, l0, l1);
+          upk2(fadd2(fadd2(sum[0], sum[1]), fadd2(sum[2], sum[3])), l0, l1);
           l += l0 + l1;
           tmem_wait_st();
           tc_fence_before();
