@@ -52,65 +52,85 @@ __device__ __forceinline__ float finish(const Params& p, int s, float sx, float 
 constexpr int FEW_WARPS = 8;
 constexpr int SEG = 64;  // bytes of K per thread quad and step
 
-// NT tiles of eight tokens, 16 output channels per block.
-template <int DT, int NT>
+// NT tiles of eight tokens, MT tiles of 16 output channels per block.
+template <int DT, int NT, int MT>
 __global__ void __launch_bounds__(FEW_WARPS * 32) gemm_few_kernel(Params p) {
   using T = typename Elem<DT>::type;
-  __shared__ int part[FEW_WARPS][NT * 8][17];
+  constexpr int CH = 16 * MT, LD = CH + 1;
+  extern __shared__ int part[];  // [FEW_WARPS][NT * 8][LD]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const int mt = (p.M + 8 * NT - 1) / (8 * NT);
-  const int n0 = (int)(blockIdx.x / mt) * 16, m0 = (int)(blockIdx.x % mt) * 8 * NT;
-  const int8_t* w0 = p.w + (size_t)::min(n0 + g, p.N - 1) * p.K;
-  const int8_t* w1 = p.w + (size_t)::min(n0 + g + 8, p.N - 1) * p.K;
+  const int n0 = (int)(blockIdx.x / mt) * CH, m0 = (int)(blockIdx.x % mt) * 8 * NT;
+  const int8_t* wr[2 * MT];
+#pragma unroll
+  for (int j = 0; j < 2 * MT; j++) wr[j] = p.w + (size_t)::min(n0 + 8 * j + g, p.N - 1) * p.K;
   const int8_t* xr[NT];
 #pragma unroll
   for (int j = 0; j < NT; j++) xr[j] = p.x + (size_t)::min(m0 + 8 * j + g, p.M - 1) * p.K;
-  int acc[NT][4] = {};
+  int acc[MT][NT][4] = {};
   const uint4 zero = make_uint4(0, 0, 0, 0);
-#pragma unroll 4
+#pragma unroll NT * MT <= 2 ? 4 : 2
   for (int k = warp * SEG + 16 * c; k < p.K + 16 * c; k += FEW_WARPS * SEG) {
     const bool in = k < p.K;  // K % 16 == 0: a 16-byte piece is inside or outside
-    const uint4 a0 = in ? __ldcs(reinterpret_cast<const uint4*>(w0 + k)) : zero;
-    const uint4 a1 = in ? __ldcs(reinterpret_cast<const uint4*>(w1 + k)) : zero;
-    const uint32_t f0[4] = {a0.x, a1.x, a0.y, a1.y}, f1[4] = {a0.z, a1.z, a0.w, a1.w};
+    uint4 a[2 * MT], b[NT];
 #pragma unroll
-    for (int j = 0; j < NT; j++) {
-      const uint4 b = in ? __ldg(reinterpret_cast<const uint4*>(xr[j] + k)) : zero;
-      mma_s8(acc[j], f0, b.x, b.y);
-      mma_s8(acc[j], f1, b.z, b.w);
+    for (int j = 0; j < 2 * MT; j++) a[j] = in ? __ldcs(reinterpret_cast<const uint4*>(wr[j] + k)) : zero;
+#pragma unroll
+    for (int j = 0; j < NT; j++) b[j] = in ? __ldg(reinterpret_cast<const uint4*>(xr[j] + k)) : zero;
+#pragma unroll
+    for (int i = 0; i < MT; i++) {
+      const uint4 a0 = a[2 * i], a1 = a[2 * i + 1];
+      const uint32_t f0[4] = {a0.x, a1.x, a0.y, a1.y}, f1[4] = {a0.z, a1.z, a0.w, a1.w};
+#pragma unroll
+      for (int j = 0; j < NT; j++) {
+        mma_s8(acc[i][j], f0, b[j].x, b[j].y);
+        mma_s8(acc[i][j], f1, b[j].z, b[j].w);
+      }
     }
   }
 #pragma unroll
-  for (int j = 0; j < NT; j++)
+  for (int i = 0; i < MT; i++)
 #pragma unroll
-    for (int i = 0; i < 4; i++) part[warp][8 * j + 2 * c + (i & 1)][g + 8 * (i >> 1)] = acc[j][i];
+    for (int j = 0; j < NT; j++)
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        part[(warp * NT * 8 + 8 * j + 2 * c + (e & 1)) * LD + 16 * i + g + 8 * (e >> 1)] = acc[i][j][e];
   __syncthreads();
   T* y = static_cast<T*>(p.y);
-  for (int i = threadIdx.x; i < NT * 8 * 16; i += FEW_WARPS * 32) {
-    const int t = i >> 4, o = i & 15;
+  for (int i = threadIdx.x; i < NT * 8 * CH; i += FEW_WARPS * 32) {
+    const int t = i / CH, o = i % CH, m = m0 + t, n = n0 + o;
+    if (m >= p.M || n >= p.N) continue;
     int s = 0;
 #pragma unroll
-    for (int k = 0; k < FEW_WARPS; k++) s += part[k][t][o];
-    const int m = m0 + t, n = n0 + o;
-    if (m < p.M && n < p.N) {
-      T* yo = y + (size_t)m * p.ld_y + n;
-      *yo = Elem<DT>::narrow(finish(p, s, __ldg(p.sx + m), __ldg(p.sw + n), p.bias ? __ldg(p.bias + n) : 0.0f,
-                                    p.ep == VXG_EP_ADD_SCALED ? Elem<DT>::widen(*yo) : 0.0f));
-    }
+    for (int k = 0; k < FEW_WARPS; k++) s += part[(k * NT * 8 + t) * LD + o];
+    T* yo = y + (size_t)m * p.ld_y + n;
+    *yo = Elem<DT>::narrow(finish(p, s, __ldg(p.sx + m), __ldg(p.sw + n), p.bias ? __ldg(p.bias + n) : 0.0f,
+                                  p.ep == VXG_EP_ADD_SCALED ? Elem<DT>::widen(*yo) : 0.0f));
   }
 }
 
-template <int DT, int NT>
-vxg_status launch_few(const Params& p, cudaStream_t st) {
-  const long long blocks = (long long)((p.M + 8 * NT - 1) / (8 * NT)) * ((p.N + 15) / 16);
+template <int DT, int NT, int MT>
+vxg_status launch_few_mt(const Params& p, cudaStream_t st) {
+  const long long blocks = (long long)((p.M + 8 * NT - 1) / (8 * NT)) * ((p.N + 16 * MT - 1) / (16 * MT));
   if (blocks > 0x7FFFFFFFLL) {
     set_error("M = %d x N = %d is more than one launch covers", p.M, p.N);
     return VXG_ERR_UNSUPPORTED;
   }
-  gemm_few_kernel<DT, NT><<<(unsigned)blocks, FEW_WARPS * 32, 0, st>>>(p);
+  constexpr int smem = FEW_WARPS * NT * 8 * (16 * MT + 1) * (int)sizeof(int);
+  const vxg_status r = smem_attr((const void*)gemm_few_kernel<DT, NT, MT>, smem);
+  if (r != VXG_OK) return r;
+  gemm_few_kernel<DT, NT, MT><<<(unsigned)blocks, FEW_WARPS * 32, smem, st>>>(p);
   note_launch();
   VXG_CUDA(cudaGetLastError());
   return VXG_OK;
+}
+
+// Every block reads all the tokens' bytes, from L2: from 17 tokens on that is as much as the weights, and a block takes
+// 32 channels to halve it, as long as that leaves a block for about every second SM.
+template <int DT, int NT>
+vxg_status launch_few(const Params& p, cudaStream_t st) {
+  if (NT >= 3 && p.N >= 2048) return launch_few_mt<DT, NT, 2>(p, st);
+  return launch_few_mt<DT, NT, 1>(p, st);
 }
 
 // ------------------------------------------------------------------------------------------------ many tokens
@@ -121,16 +141,17 @@ vxg_status launch_few(const Params& p, cudaStream_t st) {
 // Roles: warps 0-7 epilogue (TMEM lanes 32 (w % 4).., column half w / 4), warp 8 TMA producer, warp 9 MMA issuer (leader).
 namespace tc {
 
-constexpr int BM = 256, BK = 128, EPI_WARPS = 8, THREADS = (EPI_WARPS + 2) * 32;
+constexpr int BM = 256, BK = 256, SUB = 128, EPI_WARPS = 8, THREADS = (EPI_WARPS + 2) * 32;
 constexpr int GROUP_M = 8;  // token tiles that share a run of weight tiles while both stay in L2
 
 template <int BN>
 struct Cfg {
   static constexpr uint32_t A_BYTES = 128 * BK, B_BYTES = BN / 2 * BK, STAGE = A_BYTES + B_BYTES;
-  static constexpr int STAGES = BN == 256 ? 5 : BN == 128 ? 7 : 8;
+  static constexpr int STAGES = BN == 256 ? 3 : 4;       // of two swizzled runs of 128 k: a wait and a commit for 8 products
+  static constexpr uint32_t A_SUB = 128 * SUB, B_SUB = BN / 2 * SUB;
   static constexpr uint32_t COLS = 2 * BN;             // two accumulators
-  static constexpr uint32_t XCH = STAGES * STAGE;      // [8][32][33] int32: rows that cannot be stored as vectors
-  static constexpr uint32_t SCALE = XCH + EPI_WARPS * 32 * 33 * 4;  // [2][BN] channel scales, [2][BN] bias
+  static constexpr uint32_t XCH = STAGES * STAGE;      // [8][32][17] int32: rows that cannot be stored as vectors
+  static constexpr uint32_t SCALE = XCH + EPI_WARPS * 32 * 17 * 4;  // [2][BN] channel scales, [2][BN] bias
   static constexpr uint32_t BARS = SCALE + 4 * BN * 4;
   static constexpr uint32_t BYTES = BARS + (2 * STAGES + 4) * 8 + 16 + 1024;
   static_assert(BYTES <= 232448, "shared memory budget");
@@ -210,8 +231,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           if (rank == 0) mbar_arrive_expect_tx(full + s, 2 * C::STAGE);
           const uint32_t bar = map_cluster(full + s, 0);
           uint8_t* a = smem + s * C::STAGE;
-          tma_load_2d_pair(a, &map_x, c * BK, m * BM + (int)rank * 128, bar);
-          tma_load_2d_pair(a + C::A_BYTES, &map_w, c * BK, n * BN + (int)rank * (BN / 2), bar);
+#pragma unroll
+          for (int h = 0; h < BK / SUB; h++) {
+            tma_load_2d_pair(a + h * C::A_SUB, &map_x, c * BK + h * SUB, m * BM + (int)rank * 128, bar);
+            tma_load_2d_pair(a + C::A_BYTES + h * C::B_SUB, &map_w, c * BK + h * SUB, n * BN + (int)rank * (BN / 2), bar);
+          }
         }
       }
       // The copies land before the block ends: their products' commits say so; after a timeout, wait for longer than a
@@ -223,34 +247,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         for (const uint64_t t0 = globaltimer(); globaltimer() - t0 < 10000000ull;) __nanosleep(10000);
     }
   } else if (warp == EPI_WARPS + 1) {
-    if (rank == 0 && lane == 0) {
-      int it = 0, k = 0;
+    // the whole warp walks and waits, which keeps the descriptors in uniform registers; one lane issues
+    if (rank == 0) {
+      const bool leader = elect_one();
+      const uint64_t da = umma_desc_sw128(smem_u32(smem)), db = umma_desc_sw128(smem_u32(smem + C::A_BYTES));
+      int it = 0, k = 0, s = 0;
+      uint32_t phase = 0;
       bool ok = true;
       for (int t = pair; t < tiles && ok; t += pairs, k++) {
         const int b = k & 1;
-        if (k >= 2 && !wait_phase(tempty + b, ((k >> 1) - 1) & 1, status, VXG_DEV_TIMEOUT_MMA)) break;
+        ok = k < 2 || wait_phase(tempty + b, ((k >> 1) - 1) & 1, status, VXG_DEV_TIMEOUT_MMA);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
         tc_fence_after();
+        const uint32_t d = tmem + b * BN;
         for (int c = 0; c < chunks; c++, it++) {
-          const int s = it % C::STAGES;
-          if (!wait_phase(full + s, (it / C::STAGES) & 1, status, VXG_DEV_TIMEOUT_MMA)) {
-            ok = false;
-            break;
-          }
+          ok = __all_sync(0xffffffffu, wait_phase(full + s, phase, status, VXG_DEV_TIMEOUT_MMA));
+          if (!ok) break;
           tc_fence_after();
-          const uint64_t ad = umma_desc_sw128(smem_u32(smem + s * C::STAGE));
-          const uint64_t bd = umma_desc_sw128(smem_u32(smem + s * C::STAGE + C::A_BYTES));
+          const uint64_t ad = da + (uint32_t)s * (C::STAGE / 16), bd = db + (uint32_t)s * (C::STAGE / 16);
+          if (leader) {
 #pragma unroll
-          for (int j = 0; j < BK / 32; j++)
-            mma_i8_pair(tmem + b * BN, ad + 2 * j, bd + 2 * j, idesc_i8(BM, BN), (c | j) != 0 ? 1u : 0u);
-          mma_commit_pair(empty + s);
+            for (int j = 0; j < BK / 32; j++)
+              mma_i8_pair(d, ad + (j / 4) * (C::A_SUB / 16) + 2 * (j % 4), bd + (j / 4) * (C::B_SUB / 16) + 2 * (j % 4),
+                          idesc_i8(BM, BN), j != 0 || c != 0 ? 1u : 0u);
+            mma_commit_pair(empty + s);
+          }
+          __syncwarp();
+          if (++s == C::STAGES) s = 0, phase ^= 1;
         }
-        if (ok) mma_commit_pair(tfull + b);
+        if (ok && leader) mma_commit_pair(tfull + b);
+        __syncwarp();
       }
     }
   } else {
     const int q = warp & 3, half = warp >> 2, tid = threadIdx.x;
     float* sw_s = reinterpret_cast<float*>(smem + C::SCALE);
-    int* xch = reinterpret_cast<int*>(smem + C::XCH) + warp * 32 * 33;
+    int* xch = reinterpret_cast<int*>(smem + C::XCH) + warp * 32 * 17;
     T* y = static_cast<T*>(p.y);
     int k = 0;
     bool ok = true;
@@ -315,20 +348,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           }
         } else {
           // rows of any alignment: through shared memory, so that a store covers consecutive columns of one row
+          const int o = lane & 15;
 #pragma unroll
-          for (int j = 0; j < 32; j++) xch[lane * 33 + j] = (int)r[j];
-          __syncwarp();
-          const int col = n0 + c0 + lane;
-          const float swc = sw[c0 + lane], bsc = bs[c0 + lane];
-          for (int i = 0; i < 32; i++) {
-            const float sxi = __shfl_sync(0xffffffffu, sx, i);
-            if (row0 + i < p.M && col < p.N) {
-              T* yo = y + (size_t)(row0 + i) * p.ld_y + col;
-              *yo = Elem<DT>::narrow(finish(p, xch[i * 33 + lane], sxi, swc, bsc,
-                                            p.ep == VXG_EP_ADD_SCALED ? Elem<DT>::widen(*yo) : 0.0f));
+          for (int h = 0; h < 2; h++) {
+#pragma unroll
+            for (int j = 0; j < 16; j++) xch[lane * 17 + j] = (int)r[16 * h + j];
+            __syncwarp();
+            const int cc = c0 + 16 * h + o, col = n0 + cc;
+            const float swc = sw[cc], bsc = bs[cc];
+#pragma unroll 4
+            for (int i = 0; i < 32; i += 2) {
+              const int rr = i + (lane >> 4);
+              const float sxi = __shfl_sync(0xffffffffu, sx, rr);
+              if (row0 + rr < p.M && col < p.N) {
+                T* yo = y + (size_t)(row0 + rr) * p.ld_y + col;
+                *yo = Elem<DT>::narrow(finish(p, xch[rr * 17 + o], sxi, swc, bsc,
+                                              p.ep == VXG_EP_ADD_SCALED ? Elem<DT>::widen(*yo) : 0.0f));
+              }
             }
+            __syncwarp();
           }
-          __syncwarp();
         }
       }
     }
@@ -348,8 +387,8 @@ vxg_status launch(const Params& p, cudaStream_t st) {
   int* status = device_status();
   VXG_ARG(status, "no CUDA device");
   CUtensorMap mx, mw;
-  vxg_status r = make_tmap_2d_u8(&mx, p.x, (uint64_t)p.M, (uint64_t)p.K, (uint64_t)p.K, 128, BK);
-  if (r == VXG_OK) r = make_tmap_2d_u8(&mw, p.w, (uint64_t)p.N, (uint64_t)p.K, (uint64_t)p.K, BN / 2, BK);
+  vxg_status r = make_tmap_2d_u8(&mx, p.x, (uint64_t)p.M, (uint64_t)p.K, (uint64_t)p.K, 128, SUB);
+  if (r == VXG_OK) r = make_tmap_2d_u8(&mw, p.w, (uint64_t)p.N, (uint64_t)p.K, (uint64_t)p.K, BN / 2, SUB);
   if (r != VXG_OK) return r;
   const long long tiles = (long long)((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
   if (tiles > 0x3FFFFFFF) {
@@ -407,9 +446,15 @@ extern "C" vxg_status vxg_gemm_i8(const int8_t* x, const float* sx, const int8_t
     constexpr int DT = decltype(tag)::value;
     cudaStream_t st = (cudaStream_t)stream;
     if (M <= 64) {
-      r = M <= 8 ? i8::launch_few<DT, 1>(p, st)
-          : M <= 16 ? i8::launch_few<DT, 2>(p, st)
-          : M <= 32 ? i8::launch_few<DT, 4>(p, st) : i8::launch_few<DT, 8>(p, st);
+      switch ((M + 7) / 8) {
+        case 1: r = i8::launch_few<DT, 1>(p, st); break;
+        case 2: r = i8::launch_few<DT, 2>(p, st); break;
+        case 3: r = i8::launch_few<DT, 3>(p, st); break;
+        case 4: r = i8::launch_few<DT, 4>(p, st); break;
+        case 5: r = i8::launch_few<DT, 5>(p, st); break;
+        case 6: r = i8::launch_few<DT, 6>(p, st); break;
+        default: r = i8::launch_few<DT, 8>(p, st); break;
+      }
     } else {
       const int bn = i8::pick_bn(p, sm_count() / 2);
       r = bn == 256 ? i8::tc::launch<DT, 256>(p, st)
