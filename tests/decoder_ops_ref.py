@@ -88,7 +88,8 @@ def attend(cache, q, table, lens, cu, scale, causal, window, dtype):
     Per probability: f16 rounding, 11 significant bits and so at most 2^-11, and the same for a value times its scale where
     the tiles are large, 2^-10 together (f32 queries: two parts, 2^-22), and the error of its score, twice (numerator and
     denominator). A score is a sum of hd exact products in f32, in the tensor cores' order: at most (hd + 8) half-steps
-    of truncation (2^-23) of sum |q k|; exp2 and the scale products add less than 2^-20 relative for the scores' size met
+    of truncation (2^-23) of sum |q k|, and for 16-bit queries, whose codes enter as 1152 + code against a start of -1152
+    times the row's sum, of 16 partial sums of size 1152 sum |q| k_scale more; exp2 and the scale products add less than 2^-20 relative for the scores' size met
     here. A probability is rounded in units of 2^-14 of the largest value scale `ref`: f16's finest step 2^-24 there puts
     an absolute 2^-25 * 2^-14 * ref * 127 on each key's term, whatever its size. The sums over L keys: (L / 8 + 32) * 2^-23. Then one rounding to the output type: f16 results below 2^-14 are
     subnormal with steps of 2^-24, so that rounding alone is up to 2^-25 there, whatever the value."""
@@ -111,6 +112,9 @@ def attend(cache, q, table, lens, cu, scale, causal, window, dtype):
                 seen &= np.arange(L) > pos - window
             if not seen.any():
                 continue
+            biased = 0.0
+            if dtype != torch.float32:
+                biased = 16 * 2.0 ** -23 * 1152 * max(cache.scales[0][table[s][j // cache.page]].max() for j in np.flatnonzero(seen))
             for h in range(heads):
                 qq = q[cu[s] + i, h].astype(np.float64)
                 kk, vv = k[seen, h // share], v[seen, h // share]
@@ -118,6 +122,7 @@ def attend(cache, q, table, lens, cu, scale, causal, window, dtype):
                 p = np.exp(e - e.max())
                 p /= p.sum()
                 off = (hd + 8) * 2.0 ** -23 * (np.abs(kk) @ np.abs(qq) * abs(scale)).max() + 2.0 ** -21 * np.abs(e).max()
+                off += biased * np.abs(qq).sum() * abs(scale)
                 out[cu[s] + i, h] = p @ vv
                 bound[cu[s] + i, h] = ((p @ np.abs(vv)) * (prob + 2 * off + 2.0 ** -20 + (L / 8 + 32) * 2.0 ** -23) +
                                        L * 127 * 2.0 ** -39 * ref)

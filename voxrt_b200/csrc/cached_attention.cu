@@ -16,8 +16,8 @@
 // work units that is cut into equal shares, one a CTA: a CTA works off its share tile by tile, and a tile that spans
 // shares leaves partial results (maximum, sum, unnormalised row) that a second small kernel joins. Lengths are read on
 // the device, so the launch does not depend on them and can be captured; every CTA finds its share with one scan.
-//   few rows  (MT = 16): the four consumer warps take 16 keys of each block and meet at the end of a tile's share;
-//   many rows (MT = 64): each consumer warp takes 16 rows and all 64 keys.
+// This file: tiles of 64 rows, a consumer warp takes 16 rows and all 64 keys of a block. cached_attention_few.cu: up to 16
+// rows. cached_attention_tc.cu: 256 rows.
 // A fifth warp brings the codes by TMA (one box per page, 128- or 64-byte swizzle so that the operand reads below are
 // free of bank conflicts) and the scales into a ring of stages. Operand layout: the k slots of a step are permuted so
 // that a thread's operand words are consecutive codes (keys: of one key; values: one word of four keys, transposed by
@@ -33,18 +33,16 @@ namespace vxg {
 namespace catt {
 
 constexpr int BK = 64;       // keys per block
+constexpr int MT = 64;       // rows per tile, 16 a consumer warp
 constexpr int CONS = 4;      // consumer warps
 constexpr int THREADS = (CONS + 1) * 32;
-template <int HD, int MT>
+template <int HD>
 struct Layout {
   static constexpr uint32_t TILE = BK * HD;      // bytes of one block's keys or values
   static constexpr uint32_t STAGE = 2 * TILE;
-  static constexpr int STAGES = HD == 128 ? (MT == 16 ? 4 : 5) : 8;
-  static constexpr uint32_t SCALES = STAGES * STAGE;           // [stage][K 4, V 4] f32
-  static constexpr uint32_t MERGE = SCALES + STAGES * 32;      // few rows: [CONS][16][HD + 4] f32 and (max, sum)
-  static constexpr uint32_t MERGE_BYTES = MT == 16 ? CONS * 16 * (HD + 4) * 4 : 0;
-  static constexpr uint32_t STAT = MERGE + MERGE_BYTES;        // [CONS][16][2] f32
-  static constexpr uint32_t BARS = (STAT + (MT == 16 ? CONS * 16 * 8 : 0) + 15) / 16 * 16;
+  static constexpr int STAGES = HD == 128 ? 5 : 8;
+  static constexpr uint32_t SCALES = STAGES * STAGE;  // [stage][K 4, V 4] f32
+  static constexpr uint32_t BARS = SCALES + STAGES * 32;
   static constexpr uint32_t BYTES = BARS + 2 * STAGES * 8 + 1024;  // + alignment
 };
 
@@ -56,14 +54,14 @@ struct State {
   float ref;
 };
 
-template <int HD, int DT, int MT>
+template <int HD, int DT>
 __global__ void __launch_bounds__(THREADS, 2)
     attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Params p) {
-  using Lay = Layout<HD, MT>;
+  using Lay = Layout<HD>;
   using T = typename Elem<DT>::type;
   constexpr bool SPLIT = DT == VXG_DT_F32;
-  constexpr bool FEW = MT == 16;
-  constexpr int TOK = FEW ? 16 : 64;  // keys of a block that one warp takes
+  constexpr int TOK = 64;  // keys of a block that one warp takes
+  constexpr bool BIASED = !SPLIT;
   constexpr int KS = HD / 16;         // k steps of the first product
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -71,8 +69,6 @@ __global__ void __launch_bounds__(THREADS, 2)
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + Lay::BARS);
   uint64_t* empty = full + Lay::STAGES;
   __shared__ Piece first_s;  // the share's first piece
-  __shared__ Piece piece_s;  // few rows: the consumers' next one
-  __shared__ int fail;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int KV = p.c.heads, PL = p.page_log2, P = 1 << PL;  // pages are powers of two
 
@@ -82,7 +78,6 @@ __global__ void __launch_bounds__(THREADS, 2)
       mbar_init(empty + i, CONS);
     }
     fence_mbar_init();
-    fail = 0;
   }
 
   find_share<THREADS, MT, BK>(p, &first_s);
@@ -90,62 +85,7 @@ __global__ void __launch_bounds__(THREADS, 2)
   if (w.left == 0) return;
 
   if (warp == CONS) {
-    // ------------------------------------------------------------------------------------------------ producer
-    const int box = ::min(P, BK);
-    int it = 0;
-    bool ok = true;
-    for (; w.left > 0 && ok; w.next(p, MT, BK)) {
-      const Tile& t = w.t;
-      const int take = w.take(), h = w.h, off = w.off;
-      if (t.nblk > 0) {
-        int have = -1;  // first page of the 32 that the lanes hold
-        int pid = -1;
-        float ks = 0.0f, vs = 0.0f;
-        for (int b = t.blk0 + off; b < t.blk0 + off + take; b++, it++) {
-          const int pg0 = (b * BK) >> PL, npg = BK > P ? BK >> PL : 1;
-          if (have < 0 || pg0 + npg > have + 32) {
-            have = pg0;
-            const int pg = pg0 + lane;
-            pid = -1, ks = 0.0f, vs = 0.0f;
-            if ((long long)pg * P < t.kmax && (long long)(pg + 1) * P > t.kmin) {  // a page that some row sees
-              pid = __ldg(p.table + (size_t)t.s * p.max_pages + pg);
-              if (pid < 0 || pid >= p.c.n_pages) {
-                atomicCAS(p.status + 1, 0, VXG_DEV_CACHE_INDEX);
-                pid = -1;
-              } else {
-                ks = __ldg(p.c.k_scales + (size_t)pid * KV + h);
-                vs = __ldg(p.c.v_scales + (size_t)pid * KV + h);
-              }
-            }
-          }
-          const int st = it % Lay::STAGES;
-          if (it >= Lay::STAGES && !wait_phase(empty + st, ((it / Lay::STAGES) - 1) & 1, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN))
-            ok = false;
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          const int src = pg0 - have + ((lane & 3) * 16 >> PL);  // page of the block's 16-key piece lane & 3
-          const float a = __shfl_sync(0xffffffffu, ks, src & 31), v = __shfl_sync(0xffffffffu, vs, src & 31);
-          if (lane < 8) scales_s[st * 8 + lane] = lane < 4 ? a : v;
-          const unsigned valid = __ballot_sync(0xffffffffu, pid >= 0);
-          const unsigned span = npg == 32 ? ~0u : ((1u << npg) - 1u);
-          const unsigned bring = (valid >> (pg0 - have)) & span;
-          __syncwarp();
-          if (lane == 0) mbar_arrive_expect_tx(full + st, (uint32_t)__popc(bring) * box * HD * 2);
-          __syncwarp();
-          const int mypage = lane - (pg0 - have);
-          if (mypage >= 0 && mypage < npg && pid >= 0) {
-            const int row = (int)(((long long)pid * KV + h) * P) + ((b * BK) & (P - 1));
-            uint8_t* dst = smem + st * Lay::STAGE + mypage * box * HD;
-            tma_load_2d(dst, &map_k, 0, row, full + st);
-            tma_load_2d(dst + Lay::TILE, &map_v, 0, row, full + st);
-          }
-        }
-      }
-    }
-    // every copy that was issued lands before the block may end
-    const int last = ::min(it, (int)Lay::STAGES);
-    for (int i = it - last; i < it; i++)
-      wait_phase(full + i % Lay::STAGES, (i / Lay::STAGES) & 1, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN);
+    produce<HD, MT, BK, Lay::STAGES>(p, w, map_k, map_v, smem, scales_s, full, empty);
     return;
   }
 
@@ -156,10 +96,10 @@ __global__ void __launch_bounds__(THREADS, 2)
   while (w.left > 0) {
     const Tile& t = w.t;
     const int take = w.take(), h = w.h, off = w.off;
-    const int row0 = FEW ? 0 : warp * 16;  // this warp's rows of the tile
+    const int row0 = warp * 16;  // this warp's rows of the tile
     // this thread's two rows: operand fragments, limits, power of two
     uint32_t qa[KS][4], qb[SPLIT ? KS : 1][4];
-    float rowf[2];
+    float rowf[2], bias[2];
     int klo[2], khi[2];
 #pragma unroll
     for (int e = 0; e < 2; e++) {
@@ -171,7 +111,7 @@ __global__ void __launch_bounds__(THREADS, 2)
       klo[e] = p.window > 0 ? (int)::max(0LL, pos - p.window + 1) : 0;
       const T* q = static_cast<const T*>(p.q) + (long long)(t.q0 + i) * p.ld_q + (long long)head * HD + c * (HD / 4);
       float f[HD / 4];
-      float top = 0.0f;
+      float top = 0.0f, sum = 0.0f;
 #pragma unroll
       for (int d = 0; d < HD / 4; d += 8) {
         float v8[8];
@@ -194,12 +134,19 @@ __global__ void __launch_bounds__(THREADS, 2)
 #pragma unroll
       for (int w = 0; w < KS; w++) {
         const float x0 = f[4 * w] * up, x1 = f[4 * w + 1] * up, x2 = f[4 * w + 2] * up, x3 = f[4 * w + 3] * up;
-        qa[w][e] = pack_f16(x0, x1);
-        qa[w][2 + e] = pack_f16(x2, x3);
+        // a word of four codes gives the pairs (0, 2) and (1, 3) with a mask and a shift
+        qa[w][e] = pack_f16(x0, x2);
+        qa[w][2 + e] = pack_f16(x1, x3);
         if (SPLIT) {
-          qb[w][e] = pack_rest(x0, x1, qa[w][e]);
-          qb[w][2 + e] = pack_rest(x2, x3, qa[w][2 + e]);
+          qb[w][e] = pack_rest(x0, x2, qa[w][e]);
+          qb[w][2 + e] = pack_rest(x1, x3, qa[w][2 + e]);
         }
+        if (BIASED) sum = add_f16(add_f16(sum, qa[w][e]), qa[w][2 + e]);
+      }
+      if (BIASED) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        bias[e] = -1152.0f * sum;
       }
     }
     // keys that every live row of the tile sees: [all_lo, all_hi)
@@ -217,21 +164,22 @@ __global__ void __launch_bounds__(THREADS, 2)
     S.ref = 0.0f;
 
     const int nb = t.nblk > 0 ? take : 0;
-    for (int b = 0; b < nb; b++, it++) {
-      const int st = it % Lay::STAGES;
-      if (ok && !wait_phase(full + st, (it / Lay::STAGES) & 1, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN)) ok = false;
+    float inv_ref = 0.0f;
+    for (int b = 0; b < nb; b++) {
+      const int st = (it + b) % Lay::STAGES;
+      if (ok && !wait_phase(full + st, ((it + b) / Lay::STAGES) & 1, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN)) ok = false;
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       const uint8_t* kt = smem + st * Lay::STAGE;
       const uint8_t* vt = kt + Lay::TILE;
       const int key0 = (t.blk0 + off + b) * BK;
-      const int tok0 = FEW ? warp * 16 : 0;  // this warp's keys of the block
-      // ---- scores
+      constexpr int tok0 = 0;
+      // ---- scores. 16-bit queries: the codes enter as 1152 + code, and the sums begin at -1152 times the row's sum
       float s[TOK / 8][4];
 #pragma unroll
       for (int j = 0; j < TOK / 8; j++) {
 #pragma unroll
-        for (int k = 0; k < 4; k++) s[j][k] = 0.0f;
+        for (int k = 0; k < 4; k++) s[j][k] = BIASED ? bias[k >> 1] : 0.0f;
         const int r = tok0 + 8 * j + g;
         uint32_t w[HD / 16];
         if (HD == 128) {
@@ -246,7 +194,8 @@ __global__ void __launch_bounds__(THREADS, 2)
         }
 #pragma unroll
         for (int k = 0; k < KS; k++) {
-          const uint32_t b0 = codes_to_f16(__byte_perm(w[k], 0, 0x4140)), b1 = codes_to_f16(__byte_perm(w[k], 0, 0x4342));
+          const uint32_t b0 = BIASED ? codes_biased(w[k]) : codes_to_f16(w[k]);
+          const uint32_t b1 = BIASED ? codes_biased(w[k] >> 8) : codes_to_f16(w[k] >> 8);
           mma_f16(s[j], qa[k], b0, b1);
           if (SPLIT) mma_f16(s[j], qb[k], b0, b1);
         }
@@ -272,7 +221,11 @@ __global__ void __launch_bounds__(THREADS, 2)
 #pragma unroll
       for (int j = 0; j < TOK / 16; j++) vsm = fmaxf(vsm, scales_s[st * 8 + 4 + tok0 / 16 + j]);
       const float ref = fmaxf(S.ref, vsm);
-      const float reff = S.ref == ref ? 1.0f : S.ref / ref;
+      float reff = 1.0f;
+      if (ref != S.ref) {  // the same in the whole warp
+        reff = S.ref / ref;
+        inv_ref = 1.0f / ref;  // finite: a page's scale is 0 or at least 2^-126
+      }
       float alpha[2], mu[2];
 #pragma unroll
       for (int e = 0; e < 2; e++) {
@@ -295,7 +248,7 @@ __global__ void __launch_bounds__(THREADS, 2)
       // ---- probabilities and the second product, 16 keys a step
 #pragma unroll
       for (int kk = 0; kk < TOK / 16; kk++) {
-        const float vf = ref > 0.0f ? scales_s[st * 8 + 4 + tok0 / 16 + kk] / ref * 16384.0f : 0.0f;
+        const float vf = scales_s[st * 8 + 4 + tok0 / 16 + kk] * inv_ref * 16384.0f;
         uint32_t pa[4], pb[4];
 #pragma unroll
         for (int e = 0; e < 2; e++)  // key group 2 kk + e
@@ -334,10 +287,8 @@ __global__ void __launch_bounds__(THREADS, 2)
       __syncwarp();
       if (lane == 0) mbar_arrive(empty + st);
     }
-    if (!ok) {
-      // give up together: no block barrier is left hanging
-      if (lane == 0) fail = 1;
-    }
+    it += nb;
+    if (!ok) return;
 #pragma unroll
     for (int e = 0; e < 2; e++) {
       S.l[e] += __shfl_xor_sync(0xffffffffu, S.l[e], 1);
@@ -347,125 +298,67 @@ __global__ void __launch_bounds__(THREADS, 2)
     const bool whole = off == 0 && take == t.cost;
     float* part = p.part + ((size_t)blockIdx.x * MAX_PIECES + (w.first ? 0 : 1)) * MT * (HD + 2);
     // thread (g, c)'s columns: HD / 4 consecutive ones, the first HD / 8 in o[.][0 or 2], the rest in o[.][1 or 3]
-    if (FEW) {
-      float* mo = reinterpret_cast<float*>(smem + Lay::MERGE);
-      float* ms = reinterpret_cast<float*>(smem + Lay::STAT);
-#pragma unroll
-      for (int e = 0; e < 2; e++) {
-        float* row = mo + (warp * 16 + g + 8 * e) * (HD + 4) + c * (HD / 4);
-#pragma unroll
-        for (int j = 0; j < HD / 8; j++) {
-          row[j] = S.o[j][2 * e] * unit;
-          row[HD / 8 + j] = S.o[j][2 * e + 1] * unit;
-        }
-        if (c == 0) {
-          ms[(warp * 16 + g + 8 * e) * 2] = S.m[e];
-          ms[(warp * 16 + g + 8 * e) * 2 + 1] = S.l[e];
-        }
-      }
-      named_bar_sync(1, CONS * 32);
-      if (tid == 0) {  // one thread walks on for all of them, so that they always agree on the barriers to come
-        Piece n = w;
-        n.next(p, MT, BK);
-        piece_s = n;
-      }
-      for (int r = warp; r < t.rows; r += CONS) {
-        float m = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < CONS; w++) m = fmaxf(m, ms[(w * 16 + r) * 2]);
-        const float mu = m == -INFINITY ? 0.0f : m;
-        float l = 0.0f, acc[HD / 32] = {};
-#pragma unroll
-        for (int w = 0; w < CONS; w++) {
-          const float f = ex2(ms[(w * 16 + r) * 2] - mu);
-          l += f * ms[(w * 16 + r) * 2 + 1];
-#pragma unroll
-          for (int k = 0; k < HD / 32; k++) acc[k] += f * mo[(w * 16 + r) * (HD + 4) + 32 * k + lane];
-        }
-        if (whole) {
-          const int rr = t.r0 + r;
-          T* o = static_cast<T*>(p.out) + (long long)(t.q0 + rr / p.share) * p.ld_out +
-                 (long long)(h * p.share + rr % p.share) * HD;
-          const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-          for (int k = 0; k < HD / 32; k++) o[32 * k + lane] = Elem<DT>::narrow(acc[k] * inv);
-        } else {
-          float* o = part + r * (HD + 2);
-          if (lane == 0) o[0] = m, o[1] = l;
-#pragma unroll
-          for (int k = 0; k < HD / 32; k++) o[2 + 32 * k + lane] = acc[k];
-        }
-      }
-      named_bar_sync(1, CONS * 32);  // the buffers are free for the next piece
-    } else {
-#pragma unroll
-      for (int e = 0; e < 2; e++) {
-        const int r = row0 + g + 8 * e;
-        if (r >= t.rows) continue;
-        if (whole) {
-          const int rr = t.r0 + r;
-          T* o = static_cast<T*>(p.out) + (long long)(t.q0 + rr / p.share) * p.ld_out +
-                 (long long)(h * p.share + rr % p.share) * HD + c * (HD / 4);
-          const float inv = S.l[e] == 0.0f ? 0.0f : unit / S.l[e];
-#pragma unroll
-          for (int j = 0; j < HD / 8; j += 8) {
-            float a[8], b2[8];
-#pragma unroll
-            for (int k = 0; k < 8; k++) a[k] = S.o[j + k][2 * e] * inv, b2[k] = S.o[j + k][2 * e + 1] * inv;
-            store8<DT>(o + j, a);
-            store8<DT>(o + HD / 8 + j, b2);
+    #pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const int r = row0 + g + 8 * e;
+            if (r >= t.rows) continue;
+            if (whole) {
+              const int rr = t.r0 + r;
+              T* o = static_cast<T*>(p.out) + (long long)(t.q0 + rr / p.share) * p.ld_out +
+                     (long long)(h * p.share + rr % p.share) * HD + c * (HD / 4);
+              const float inv = S.l[e] == 0.0f ? 0.0f : unit / S.l[e];
+    #pragma unroll
+              for (int j = 0; j < HD / 8; j += 8) {
+                float a[8], b2[8];
+    #pragma unroll
+                for (int k = 0; k < 8; k++) a[k] = S.o[j + k][2 * e] * inv, b2[k] = S.o[j + k][2 * e + 1] * inv;
+                store8<DT>(o + j, a);
+                store8<DT>(o + HD / 8 + j, b2);
+              }
+            } else {
+              float* o = part + r * (HD + 2);
+              if (c == 0) o[0] = S.m[e], o[1] = S.l[e];
+              o += 2 + c * (HD / 4);
+    #pragma unroll
+              for (int j = 0; j < HD / 8; j++) {
+                o[j] = S.o[j][2 * e] * unit;
+                o[HD / 8 + j] = S.o[j][2 * e + 1] * unit;
+              }
+            }
           }
-        } else {
-          float* o = part + r * (HD + 2);
-          if (c == 0) o[0] = S.m[e], o[1] = S.l[e];
-          o += 2 + c * (HD / 4);
-#pragma unroll
-          for (int j = 0; j < HD / 8; j++) {
-            o[j] = S.o[j][2 * e] * unit;
-            o[HD / 8 + j] = S.o[j][2 * e + 1] * unit;
-          }
-        }
-      }
-    }
-    if (FEW) {
-      if (fail) return;  // set before the first of the two barriers above
-      w = piece_s;
-    } else {
-      if (!ok) return;
-      w.next(p, MT, BK);
-    }
+    w.next(p, MT, BK);
   }
 }
 
 constexpr int CTAS_PER_SM = 2;
 
-// The three kernels by the average number of (query, query head) rows a sequence and KV head has: up to 16 rows, tiles of
-// 16; up to 96, tiles of 64; beyond, tiles of 256 on tcgen05 (16-bit queries).
+// The kernels by the average number of (query, query head) rows a sequence and KV head has: up to 8 and 16 rows, tiles
+// of as many; up to 96, tiles of 64; beyond, tiles of 256 on tcgen05 (16-bit queries).
 static vxg_status plan(int total, int n_seq, int heads, int kv, int hd, int dtype, Plan* pl) {
   const long long share = heads / kv, rows = (long long)total * share;
-  pl->mt = rows <= 16LL * n_seq ? 16 : rows <= 96LL * n_seq || dtype == VXG_DT_F32 ? 64 : 256;
+  pl->mt = rows <= 8LL * n_seq ? 8 : rows <= 16LL * n_seq ? 16 : rows <= 96LL * n_seq || dtype == VXG_DT_F32 ? 64 : 256;
   const long long slots = rows / pl->mt + n_seq;
   if (slots > 0x3FFFFFFF) {
     set_error("%d rows of %d heads are more than one launch covers", total, heads);
     return VXG_ERR_UNSUPPORTED;
   }
   pl->slots = (int)slots;
-  pl->grid = sm_count() * (pl->mt == 256 ? 1 : CTAS_PER_SM);
+  pl->grid = sm_count() * (pl->mt == 256 ? 1 : pl->mt == 8 ? FEW_CTAS_8 : CTAS_PER_SM);
   pl->rec_bytes = (size_t)pl->grid * 8 * sizeof(long long);
   pl->part_bytes = (size_t)pl->grid * MAX_PIECES * pl->mt * (hd + 2) * sizeof(float);
   return VXG_OK;
 }
 
-template <int HD, int DT, int MT>
+template <int HD, int DT>
 vxg_status launch(const Params& p, const Plan& pl, cudaStream_t st) {
   CUtensorMap mk, mv;
   vxg_status r = cache_map(&mk, p.c, p.c.k, BK);
   if (r == VXG_OK) r = cache_map(&mv, p.c, p.c.v, BK);
   if (r != VXG_OK) return r;
-  constexpr int smem = (int)Layout<HD, MT>::BYTES;
+  constexpr int smem = (int)Layout<HD>::BYTES;
   static_assert((smem + 1024) * CTAS_PER_SM <= 228 * 1024, "two blocks share an SM");
-  if ((r = smem_attr((const void*)attend_kernel<HD, DT, MT>, smem)) != VXG_OK) return r;
-  attend_kernel<HD, DT, MT><<<pl.grid, THREADS, smem, st>>>(mk, mv, p);
+  if ((r = smem_attr((const void*)attend_kernel<HD, DT>, smem)) != VXG_OK) return r;
+  attend_kernel<HD, DT><<<pl.grid, THREADS, smem, st>>>(mk, mv, p);
   VXG_CUDA(cudaGetLastError());
   join_kernel<HD, DT, MT, BK><<<dim3(pl.grid - 1, MT / 4), 128, 0, st>>>(p);
   note_launch(2);
@@ -522,10 +415,10 @@ vxg_status vxg_cache_attention(const vxg_kv_cache* c, const void* q, long long l
   p.scale_log2 = scale * 1.44269504088896340736f;
   cudaStream_t st = (cudaStream_t)stream;
   if (pl.mt == 256) return catt::launch_tc(p, pl, c->head_dim, dtype, st);
+  if (pl.mt <= 16) return catt::launch_few(p, pl, c->head_dim, dtype, st);
   with_dtype(dtype, [&](auto tag) {
     constexpr int DT = decltype(tag)::value;
-    if (c->head_dim == 128) r = pl.mt == 16 ? catt::launch<128, DT, 16>(p, pl, st) : catt::launch<128, DT, 64>(p, pl, st);
-    else r = pl.mt == 16 ? catt::launch<64, DT, 16>(p, pl, st) : catt::launch<64, DT, 64>(p, pl, st);
+    r = c->head_dim == 128 ? catt::launch<128, DT>(p, pl, st) : catt::launch<64, DT>(p, pl, st);
   });
   return r;
 }

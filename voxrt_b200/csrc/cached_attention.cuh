@@ -35,6 +35,9 @@ struct Plan {
   size_t rec_bytes, part_bytes;
 };
 
+constexpr int FEW_CTAS_8 = 3;  // CTAs an SM, tiles of up to 8 rows
+// Tiles of up to 16 rows (cached_attention_few.cu).
+vxg_status launch_few(const Params& p, const Plan& pl, int head_dim, int dtype, cudaStream_t st);
 // 256-row tiles on tcgen05, f16 and bf16 queries (cached_attention_tc.cu).
 vxg_status launch_tc(const Params& p, const Plan& pl, int head_dim, int dtype, cudaStream_t st);
 
@@ -183,6 +186,70 @@ __device__ __forceinline__ void find_share(const Params& p, Piece* first_s) {
   if (tid == 0 && first_s->left == 0) p.rec[blockIdx.x * 8] = -1;  // more CTAs than units
 }
 
+// One warp brings the share's blocks of BK keys: codes [K BK x HD][V BK x HD] by TMA, one box per page, into a ring of
+// STAGES stages, and the scales of a block's 16-key pieces (four of K, four of V) beside it. Pages and scales are looked
+// up 32 pages at a time. Pages that no row of the tile sees are not brought and have scale 0.
+template <int HD, int MT, int BK, int STAGES>
+__device__ __forceinline__ void produce(const Params& p, Piece w, const CUtensorMap& map_k, const CUtensorMap& map_v,
+                                        uint8_t* smem, float* scales_s, uint64_t* full, uint64_t* empty) {
+  const int lane = threadIdx.x & 31, KV = p.c.heads, PL = p.page_log2, P = 1 << PL;
+  const int box = ::min(P, BK);
+  int it = 0;
+  bool ok = true;
+  for (; w.left > 0 && ok; w.next(p, MT, BK)) {
+    const Tile& t = w.t;
+    const int take = w.take(), h = w.h, off = w.off;
+    if (t.nblk > 0) {
+      int have = -1;  // first page of the 32 that the lanes hold
+      int pid = -1;
+      float ks = 0.0f, vs = 0.0f;
+      for (int b = t.blk0 + off; b < t.blk0 + off + take; b++, it++) {
+        const int pg0 = (b * BK) >> PL, npg = BK > P ? BK >> PL : 1;
+        if (have < 0 || pg0 + npg > have + 32) {
+          have = pg0;
+          const int pg = pg0 + lane;
+          pid = -1, ks = 0.0f, vs = 0.0f;
+          if ((long long)pg * P < t.kmax && (long long)(pg + 1) * P > t.kmin) {  // a page that some row sees
+            pid = __ldg(p.table + (size_t)t.s * p.max_pages + pg);
+            if (pid < 0 || pid >= p.c.n_pages) {
+              atomicCAS(p.status + 1, 0, VXG_DEV_CACHE_INDEX);
+              pid = -1;
+            } else {
+              ks = __ldg(p.c.k_scales + (size_t)pid * KV + h);
+              vs = __ldg(p.c.v_scales + (size_t)pid * KV + h);
+            }
+          }
+        }
+        const int st = it % STAGES;
+        if (it >= STAGES && !wait_phase(empty + st, ((it / STAGES) - 1) & 1, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN))
+          ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const int src = pg0 - have + ((lane & 3) * 16 >> PL);  // page of the block's 16-key piece lane & 3
+        const float a = __shfl_sync(0xffffffffu, ks, src & 31), v = __shfl_sync(0xffffffffu, vs, src & 31);
+        if (lane < 8) scales_s[st * 8 + lane] = lane < 4 ? a : v;
+        const unsigned valid = __ballot_sync(0xffffffffu, pid >= 0);
+        const unsigned span = npg == 32 ? ~0u : ((1u << npg) - 1u);
+        const unsigned bring = (valid >> (pg0 - have)) & span;
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect_tx(full + st, (uint32_t)__popc(bring) * box * HD * 2);
+        __syncwarp();
+        const int mypage = lane - (pg0 - have);
+        if (mypage >= 0 && mypage < npg && pid >= 0) {
+          const int row = (int)(((long long)pid * KV + h) * P) + ((b * BK) & (P - 1));
+          uint8_t* dst = smem + st * (2 * BK * HD) + mypage * box * HD;
+          tma_load_2d(dst, &map_k, 0, row, full + st);
+          tma_load_2d(dst + BK * HD, &map_v, 0, row, full + st);
+        }
+      }
+    }
+  }
+  // every copy that was issued lands before the block may end
+  const int last = ::min(it, (int)STAGES);
+  for (int i = it - last; i < it; i++)
+    wait_phase(full + i % STAGES, (i / STAGES) & 1, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN);
+}
+
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -192,8 +259,9 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
 
 // Two int8 codes in bytes 0 and 2 of w -> two f16. Flipping a code's sign bit adds 128, and 0x64 above it makes the
 // f16 1024 + 128 + code, exactly.
+__device__ __forceinline__ uint32_t codes_biased(uint32_t w) { return (w & 0x00FF00FFu) ^ 0x64806480u; }
 __device__ __forceinline__ uint32_t codes_to_f16(uint32_t w) {
-  const uint32_t biased = (w & 0x00FF00FFu) ^ 0x64806480u;
+  const uint32_t biased = codes_biased(w);
   const uint32_t off = 0x64806480u;  // 1152, 1152
   const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&biased), *reinterpret_cast<const __half2*>(&off));
   return *reinterpret_cast<const uint32_t*>(&r);
@@ -202,6 +270,11 @@ __device__ __forceinline__ uint32_t codes_to_f16(uint32_t w) {
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+// sum plus the two f16 of h
+__device__ __forceinline__ float add_f16(float sum, uint32_t h) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+  return sum + f.x + f.y;
 }
 // the part of (a, b) that pack_f16 leaves out
 __device__ __forceinline__ uint32_t pack_rest(float a, float b, uint32_t hi) {
