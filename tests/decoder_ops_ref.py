@@ -90,8 +90,9 @@ def attend(cache, q, table, lens, cu, scale, causal, window, dtype):
     denominator). A score is a sum of hd exact products in f32, in the tensor cores' order: at most (hd + 8) half-steps
     of truncation (2^-23) of sum |q k|, and for 16-bit queries, whose codes enter as 1152 + code against a start of -1152
     times the row's sum, of 16 partial sums of size 1152 sum |q| k_scale more; exp2 and the scale products add less than 2^-20 relative for the scores' size met
-    here. A probability is rounded in units of 2^-14 of the largest value scale `ref`: f16's finest step 2^-24 there puts
-    an absolute 2^-25 * 2^-14 * ref * 127 on each key's term, whatever its size. The sums over L keys: (L / 8 + 32) * 2^-23. Then one rounding to the output type: f16 results below 2^-14 are
+    here. A probability is rounded in units of 2^-7 (at the coarsest) of the largest value scale `ref`: f16's finest step
+    2^-24 there puts an absolute 2^-25 * 2^-7 * ref * 127 on each key's term, whatever its size, against a sum of at
+    least 1. The sums over L keys: (L / 8 + 32) * 2^-23. Then one rounding to the output type: f16 results below 2^-14 are
     subnormal with steps of 2^-24, so that rounding alone is up to 2^-25 there, whatever the value."""
     rows, heads, hd = q.shape
     share = heads // cache.heads
@@ -125,5 +126,5 @@ def attend(cache, q, table, lens, cu, scale, causal, window, dtype):
                 off += biased * np.abs(qq).sum() * abs(scale)
                 out[cu[s] + i, h] = p @ vv
                 bound[cu[s] + i, h] = ((p @ np.abs(vv)) * (prob + 2 * off + 2.0 ** -20 + (L / 8 + 32) * 2.0 ** -23) +
-                                       L * 127 * 2.0 ** -39 * ref)
+                                       L * 127 * 2.0 ** -32 * ref)
     return out, bound + HALF[dtype] * (np.abs(out) + bound) + (2.0 ** -25 if dtype == torch.float16 else 1e-30)

@@ -9,7 +9,7 @@
 // power of two, `scale` and log2(e) multiply the f32 sum. The softmax is kept in f32 with a running maximum and sum;
 // a probability enters the second product as f16(p * 2^14 * v_scale / ref), ref being the largest value scale met so
 // far (rounding 2^-11 of each term at most, 2^-39 absolute against the largest; two parts for f32), and ref and 2^-14 multiply
-// the result. The sum of the row is taken from the unrounded p.
+// the result. (The kernels for few and many rows let the maximum lag by up to 2^8 and use 2^7 for 2^14.) The sum of the row is taken from the unrounded p.
 //
 // Work split. A tile is MT consecutive (query, query head) rows of one sequence and KV head, so a key is read once for
 // all the query heads that share it. The keys it sees, in blocks of 64, times all tiles and KV heads form one line of

@@ -72,7 +72,8 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? FEW_CTAS_8 : 2)
   }
 
   const int g = lane >> 2, c = lane & 3;
-  int it = 0;
+  int st = 0;
+  uint32_t phase = 0;
   bool ok = true;
   while (w.left > 0) {
     const Tile& t = w.t;
@@ -135,10 +136,13 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? FEW_CTAS_8 : 2)
         klo[n][e] = __shfl_sync(0xffffffffu, lo, src);
       }
     }
-    // keys that every live row of the tile sees: [all_lo, all_hi)
+    const int nb = t.nblk > 0 ? take : 0, blk = t.blk0 + off;
+    // blocks [in0, in1) of the piece: every live row of the tile sees all of their keys
     const int last_i = (t.r0 + t.rows - 1) / p.share, first_i = t.r0 / p.share;
     const long long all_hi = p.causal ? (long long)t.L - t.n + first_i + 1 : t.L;
     const long long all_lo = p.window > 0 ? (long long)t.L - t.n + last_i - p.window + 1 : 0;
+    const int in0 = (int)::min((long long)nb, ::max(0LL, (all_lo + BK - 1) / BK - blk));
+    const int in1 = (int)::min((long long)nb, ::max((long long)in0, all_hi > 0 ? all_hi / BK - blk : 0LL));
 
     float o[NQ][KS][4], m[NQ][2], l[NQ][2];  // o[n][i]: columns HD/8 g + 2 i (0, 1) and the next (2, 3), rows 2 c and 2 c + 1
     float ref = 0.0f, inv_ref = 0.0f;
@@ -152,15 +156,11 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? FEW_CTAS_8 : 2)
       l[n][0] = l[n][1] = 0.0f;
     }
 
-    const int nb = t.nblk > 0 ? take : 0;
-    for (int b = 0; b < nb; b++, it++) {
-      const int st = it % Lay::STAGES;
-      if (ok && !wait_phase(full + st, (it / Lay::STAGES) & 1, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN)) ok = false;
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
+    auto block = [&](auto tag, int b) {
+      constexpr bool masked = decltype(tag)::value;
       const uint8_t* kt = smem + st * Lay::STAGE;
       const uint8_t* vt = kt + BK * HD;
-      const int key0 = (t.blk0 + off + b) * BK, tok0 = warp * 16;
+      const int tok0 = warp * 16, key0 = (blk + b) * BK + tok0 + g;
       const float ks = scales_s[st * 8 + warp], vs = scales_s[st * 8 + 4 + warp];
       // ---- scores of keys tok0 + g and tok0 + g + 8
       float s[NQ][4];
@@ -211,60 +211,66 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? FEW_CTAS_8 : 2)
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(empty + st);
-      // ---- scale, mask, running maximum
-      const bool inside = key0 >= all_lo && key0 + BK <= all_hi;
-      const float ref1 = fmaxf(ref, vs);
-      float reff = 1.0f;
-      if (ref1 != ref) {  // the same in the whole warp
-        reff = ref / ref1;
-        inv_ref = 1.0f / ref1;  // finite: a page's scale is 0 or at least 2^-126
-        ref = ref1;
+      // ---- scale, mask
+      bool over = false;
+#pragma unroll
+      for (int n = 0; n < NQ; n++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const int e = k & 1;
+          s[n][k] = (s[n][k] + s2[n][k]) * (rowf[n][e] * ks);
+          if (masked) {
+            const int key = key0 + (k >> 1) * 8;
+            if (key < klo[n][e] || key >= khi[n][e]) s[n][k] = -INFINITY;
+          }
+          over = over || s[n][k] > m[n][e] + 8.0f;
+        }
+      // ---- the rows' references move when a score has outgrown one by 2^8, ref when a value scale is larger than all before
+      const bool wider = vs > ref;
+      if (__any_sync(0xffffffffu, over || wider)) {
+        float reff = 1.0f;
+        if (wider) {  // the same in the whole warp
+          reff = ref / vs;
+          inv_ref = 128.0f / vs;  // finite: a page's scale is 0 or at least 2^-126
+          ref = vs;
+        }
+#pragma unroll
+        for (int n = 0; n < NQ; n++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            float mx = fmaxf(s[n][e], s[n][2 + e]);
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            mx = fmaxf(mx, m[n][e]);
+            const float a = ex2(m[n][e] - (mx == -INFINITY ? 0.0f : mx));
+            m[n][e] = mx;
+            l[n][e] *= a;
+#pragma unroll
+            for (int i = 0; i < KS; i++) o[n][i][e] *= a * reff, o[n][i][2 + e] *= a * reff;
+          }
       }
-      const float vf = vs * inv_ref * 16384.0f;
-      bool same = true;
-      float alpha[NQ][2];
+      // ---- probabilities, times 2^7 and the value scale for the second product
+      const float vf = vs * inv_ref;
       uint32_t pb[NQ][2], pr[SPLIT ? NQ : 1][2];
 #pragma unroll
       for (int n = 0; n < NQ; n++) {
         float pv[4];
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-          const float f = rowf[n][e] * ks;
-          float y0 = (s[n][e] + s2[n][e]) * f, y1 = (s[n][2 + e] + s2[n][2 + e]) * f;
-          if (!inside) {
-            const int k0 = key0 + tok0 + g;
-            if (k0 < klo[n][e] || k0 >= khi[n][e]) y0 = -INFINITY;
-            if (k0 + 8 < klo[n][e] || k0 + 8 >= khi[n][e]) y1 = -INFINITY;
-          }
-          float mx = fmaxf(y0, y1);
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          mx = fmaxf(mx, m[n][e]);
-          const float mu = mx == -INFINITY ? 0.0f : mx;
-          const float a = ex2(m[n][e] - mu);
-          m[n][e] = mx;
-          const float p0 = ex2(y0 - mu), p1 = ex2(y1 - mu);
-          l[n][e] = l[n][e] * a + (p0 + p1);
-          alpha[n][e] = a * reff;
-          same = same && alpha[n][e] == 1.0f;
-          pv[e] = p0 * vf;
-          pv[2 + e] = p1 * vf;
+        for (int k = 0; k < 4; k++) {
+          const float mu = m[n][k & 1] == -INFINITY ? 0.0f : m[n][k & 1];
+          pv[k] = ex2(s[n][k] - mu);
         }
+        l[n][0] += pv[0] + pv[2];
+        l[n][1] += pv[1] + pv[3];
+#pragma unroll
+        for (int k = 0; k < 4; k++) pv[k] *= vf;
 #pragma unroll
         for (int k = 0; k < 2; k++) {
           const uint32_t hi = pack_f16(pv[2 * k], pv[2 * k + 1]);
           pb[n][k] = transpose8(hi);
           if (SPLIT) pr[n][k] = transpose8(pack_rest(pv[2 * k], pv[2 * k + 1], hi));
         }
-      }
-      if (!__all_sync(0xffffffffu, same)) {
-#pragma unroll
-        for (int n = 0; n < NQ; n++)
-#pragma unroll
-          for (int i = 0; i < KS; i++)
-#pragma unroll
-            for (int k = 0; k < 4; k++) o[n][i][k] *= alpha[n][k & 1];
       }
       // ---- the second product: row tile i holds columns 2 i and 2 i + 1 of every g's run
 #pragma unroll
@@ -278,10 +284,17 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? FEW_CTAS_8 : 2)
           if (SPLIT) mma_f16(o[n][i], a, pr[n][0], pr[n][1]);
         }
       }
+    };
+    for (int b = 0; b < nb; b++) {
+      ok = __all_sync(0xffffffffu, wait_phase(full + st, phase, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN));
+      if (!ok) break;
+      if (b >= in0 && b < in1) block(std::false_type(), b);
+      else block(std::true_type(), b);
+      if (++st == Lay::STAGES) st = 0, phase ^= 1;
     }
     if (!ok && lane == 0) fail = 1;  // read behind the second barrier below: all give up together
     // ---- the warps' states meet
-    const float unit = ref * (1.0f / 16384.0f);
+    const float unit = ref * (1.0f / 128.0f);
     const bool whole = off == 0 && take == t.cost;
     float* part = p.part + ((size_t)blockIdx.x * MAX_PIECES + (w.first ? 0 : 1)) * MT * (HD + 2);
     float* mo = reinterpret_cast<float*>(smem + Lay::MERGE);
