@@ -360,10 +360,7 @@ vxg_status launch(const Params& p, const Plan& pl, cudaStream_t st) {
   if ((r = smem_attr((const void*)attend_kernel<HD, DT>, smem)) != VXG_OK) return r;
   attend_kernel<HD, DT><<<pl.grid, THREADS, smem, st>>>(mk, mv, p);
   VXG_CUDA(cudaGetLastError());
-  join_kernel<HD, DT, MT, BK><<<dim3(pl.grid - 1, MT / 4), 128, 0, st>>>(p);
-  note_launch(2);
-  VXG_CUDA(cudaGetLastError());
-  return VXG_OK;
+  return launch_join<HD, DT, MT, BK>(p, pl, st);
 }
 
 }  // namespace catt

@@ -23,7 +23,7 @@ struct Params {
   const int* len;
   const int* cu;
   float* part;      // [grid][2][MT][HD + 2]
-  long long* rec;   // [grid][8]: begin, first unit and end of the tile it lies in, slot of the batch, KV head
+  long long* rec;   // [grid][8]: begin, first unit and end of the tile it lies in, slot of the batch, KV head, all units, shares
   int* status;
   int n_seq, max_pages, total, heads, share, window, causal, slots, grid;
   int page_log2;
@@ -134,6 +134,7 @@ __device__ __forceinline__ void find_share(const Params& p, Piece* first_s) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int KV = p.c.heads;
   if (tid == 0) first_s->left = 0;
+  grid_launch_dependents();  // the join, which waits for this kernel's end
   const int per = (p.slots + THREADS - 1) / THREADS;
   const int sl0 = ::min(p.slots, tid * per), sl1 = ::min(p.slots, sl0 + per);
   const int first_seq = sl0 < sl1 ? find_seq(p, sl0, MT) : 0;
@@ -175,7 +176,7 @@ __device__ __forceinline__ void find_share(const Params& p, Piece* first_s) {
           first_s->left = end - begin;
           first_s->first = 1;
           long long* r = p.rec + blockIdx.x * 8;
-          r[0] = begin, r[1] = begin - first_s->off, r[2] = r[1] + t.cost, r[3] = i, r[4] = first_s->h, r[5] = end;
+          r[0] = begin, r[1] = begin - first_s->off, r[2] = r[1] + t.cost, r[3] = i, r[4] = first_s->h, r[5] = units, r[6] = parts;
           break;
         }
         at += t.cost;
@@ -295,6 +296,7 @@ __global__ void __launch_bounds__(128) join_kernel(const Params p) {
   using T = typename Elem<DT>::type;
   constexpr int N = HD / 32;
   const int b = blockIdx.x + 1, lane = threadIdx.x & 31, r = blockIdx.y * 4 + (threadIdx.x >> 5);
+  grid_wait();  // launched while the kernel in front still runs
   const long long* rec = p.rec + (size_t)b * 8;
   const long long begin = rec[0];
   if (begin < 0) return;
@@ -309,8 +311,8 @@ __global__ void __launch_bounds__(128) join_kernel(const Params p) {
     const int k = j == b - 1 && prev != u0 ? 1 : 0;
     return p.part + ((size_t)j * MAX_PIECES + k) * MT * (HD + 2) + (size_t)r * (HD + 2);
   };
-  int last = b;  // shares b - 1 .. last hold parts of the tile
-  while (last + 1 < p.grid && p.rec[(size_t)last * 8 + 5] < u1) last++;
+  // shares b - 1 .. last hold parts of the tile: share j begins at floor(units j / parts), and last is the one of unit u1 - 1
+  const int last = (int)((u1 * rec[6] + rec[5] - 1) / rec[5]) - 1;
   float m = -INFINITY;
   for (int j = b - 1 + lane; j <= last; j += 32) m = fmaxf(m, at(j)[0]);
 #pragma unroll
@@ -331,6 +333,24 @@ __global__ void __launch_bounds__(128) join_kernel(const Params p) {
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
   for (int k = 0; k < N; k++) o[32 * k + lane] = Elem<DT>::narrow(acc[k] * inv);
+}
+
+// The join is put behind its kernel with the launch's latency hidden under it (its blocks wait for the kernel's end).
+template <int HD, int DT, int MT, int BK>
+vxg_status launch_join(const Params& p, const Plan& pl, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(pl.grid - 1, MT / 4);
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  VXG_CUDA(cudaLaunchKernelEx(&cfg, join_kernel<HD, DT, MT, BK>, p));
+  note_launch(2);
+  VXG_CUDA(cudaGetLastError());
+  return VXG_OK;
 }
 
 }  // namespace catt

@@ -363,10 +363,7 @@ vxg_status launch(const Params& p, const Plan& pl, cudaStream_t st) {
   if ((r = smem_attr((const void*)attend_few_kernel<HD, DT, NQ>, smem)) != VXG_OK) return r;
   attend_few_kernel<HD, DT, NQ><<<pl.grid, THREADS, smem, st>>>(mk, mv, p);
   VXG_CUDA(cudaGetLastError());
-  join_kernel<HD, DT, 8 * NQ, BK><<<dim3(pl.grid - 1, 2 * NQ), 128, 0, st>>>(p);
-  note_launch(2);
-  VXG_CUDA(cudaGetLastError());
-  return VXG_OK;
+  return launch_join<HD, DT, 8 * NQ, BK>(p, pl, st);
 }
 
 }  // namespace few

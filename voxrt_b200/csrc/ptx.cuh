@@ -368,6 +368,11 @@ __device__ __forceinline__ void bulk_wait_read_1() {
 // Wait until every committed bulk store of this thread has completed.
 __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
+// Programmatic dependent launch: let the next kernel's blocks start, / wait until the kernel in front has ended and its
+// writes are visible.
+__device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---------------------------------------------------------------------------- pairs of CTAs (cta_group::2)
 
 __device__ __forceinline__ uint32_t cluster_rank() {
