@@ -100,6 +100,25 @@ def test_quantize_and_back(K, n, d, group, dtype):
     assert (err <= s[..., None] * (0.5 + 127 * 3 * HALF[torch.float32])).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantize_non_finite_tiny_and_huge(K, dtype):
+    """Per group: NaN gives code 0 and the others keep their scale; an infinity makes the group's scale infinite; values
+    at either end of the type; all in one call, next to ordinary groups."""
+    x = torch.randn((6, 1280), generator=torch.Generator().manual_seed(3)).to(dtype)
+    x[0, ::7] = float("nan")
+    x[1, 130] = float("inf")
+    x[2, 256:384] *= torch.finfo(dtype).smallest_normal
+    x[3, :128] = torch.finfo(dtype).max
+    x[4, 128:256] = float("nan")
+    x[5, 640:768] = 0
+    wide = torch.empty((6, 1288), dtype=dtype, device="cuda")[:, :1280]
+    wide.copy_(x)
+    for group in (128, 1280, 320):
+        q, s = quant(f32(x), group)
+        a = K.quantize(wide, group)
+        assert np.array_equal(a.x.cpu().numpy(), q) and bits_equal(f32(a.scales), s)
+
+
 def test_existing_quantizer_agrees(K):
     x = torch.randn((33, 1024), generator=torch.Generator().manual_seed(7)).cuda()
     wide = torch.empty((33, 1030), device="cuda")[:, :1024]
