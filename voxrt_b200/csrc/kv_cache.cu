@@ -8,8 +8,9 @@
 // A scale only grows while a page fills, so a token written alone is off by at most half a step of the page's final
 // scale plus half a step for each growth after it.
 //
-// Bound by memory: one block takes one (page, head) of K or V. The values are read twice, the second time from L1 / L2
-// (at most 32 KB of 16-bit values a block).
+// Bound by memory for long runs, by the chain of dependent loads (offsets, page table, values) for single tokens: one
+// block takes one page of K or V and a run of heads, finds its sequence with 32 probes a step, and holds a head's new values
+// in registers between the maximum and the codes, with the next head's on their way.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -22,7 +23,6 @@
 namespace vxg {
 namespace cache {
 
-constexpr int THREADS = 128;
 
 struct WriteParams {
   vxg_kv_cache c;
@@ -32,7 +32,7 @@ struct WriteParams {
   const int* start;
   const int* cu;
   int* status;
-  int total, n_seq, max_pages;
+  int total, n_seq, max_pages, run;  // run: heads of a block
 };
 
 __device__ __forceinline__ float finite_abs(float v) {
@@ -43,23 +43,33 @@ __device__ __forceinline__ float finite_abs(float v) {
 // code of v under inv = 1 / s: an infinity is the largest code (inv > 0), a NaN 0
 __device__ __forceinline__ uint32_t code8(float v, float inv) { return (uint32_t)quant_code(v, inv) & 0xFFu; }
 
+// Largest i < n with at(i) <= x, or 0; `at` does not decrease. Every lane of the warp asks for the same x.
+template <class At>
+__device__ __forceinline__ int find32(int n, long long x, At at) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0;
+  while (n > 1) {
+    const int step = (n + 31) / 32, i = lane * step;
+    const unsigned below = __ballot_sync(0xffffffffu, i < n && at(lo + i) <= x);
+    const int k = below ? 31 - __clz(below) : 0;
+    lo += k * step;
+    n = ::min(step, n - k * step);
+  }
+  return lo;
+}
+
 // Pages of sequence s in the launch's item order: at most (cu[s+1] - cu[s] - 2) / page + 2 of them are touched, and
 // items base(s) .. base(s + 1) with base(s) = cu[s] / page + 2 s are as many or more, so that total / page + 2 n_seq
-// items cover every batch without the host knowing its lengths.
-template <int DT, bool VEC>
-__global__ void __launch_bounds__(THREADS) cache_write_kernel(WriteParams p) {
+// items cover every batch without the host knowing its lengths. NV: vectors of eight values a thread holds; with fewer
+// threads than that covers (LONG) the rest is read twice.
+template <int DT, int THREADS, int NV, bool VEC, bool LONG>
+__global__ void __launch_bounds__(THREADS) cache_write_kernel(const WriteParams p) {
   using T = typename Elem<DT>::type;
-  __shared__ float wmax[THREADS / 32];
+  __shared__ float wmax[2][THREADS / 32];
   const int P = p.c.page, H = p.c.heads, D = p.c.head_dim;
-  const int item = blockIdx.x, h = blockIdx.y, which = blockIdx.z;
-  auto base = [&](int s) { return (long long)__ldg(p.cu + s) / P + 2LL * s; };
-  int lo = 0, hi = p.n_seq;  // largest s with base(s) <= item
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (base(mid) <= item) lo = mid;
-    else hi = mid;
-  }
-  const int s = lo;
+  const int item = blockIdx.x, which = blockIdx.z, h0 = blockIdx.y * p.run, h1 = ::min(H, h0 + p.run);
+  auto base = [&](int s) { return (long long)(__ldg(p.cu + s) / P) + 2LL * s; };
+  const int s = find32(p.n_seq, item, base);
   const int t0 = __ldg(p.cu + s), n = __ldg(p.cu + s + 1) - t0;
   if (n == 0) return;
   const long long a = __ldg(p.start + s);
@@ -68,24 +78,17 @@ __global__ void __launch_bounds__(THREADS) cache_write_kernel(WriteParams p) {
     if (threadIdx.x == 0) atomicCAS(p.status + 1, 0, VXG_DEV_CACHE_INDEX);
     return;
   }
-  const long long pg = a / P + (item - base(s));  // page of the sequence
-  if (item < base(s) || pg * P >= a + n) return;
+  const int first = (int)a / P, pg = first + (int)(item - base(s));  // page of the sequence; a + n < 2^31
+  if (pg < first || (long long)pg * P >= a + n) return;
   const int pid = __ldg(p.table + (size_t)s * p.max_pages + pg);
-  if (pid < 0 || pid >= p.c.n_pages) {
-    if (threadIdx.x == 0) atomicCAS(p.status + 1, 0, VXG_DEV_CACHE_INDEX);
-    return;
-  }
-  const int held = a > pg * P ? (int)(a - pg * P) : 0;                // earlier tokens of the sequence in this page
-  const int end = (int)(a + n < (pg + 1) * P ? a + n - pg * P : P);   // new tokens: slots held .. end
-  const long long tok = t0 + (pg * P + held - a);                     // stacked row of slot `held`
-  const size_t ph = (size_t)pid * H + h;
-  float* scale = (which ? p.c.v_scales : p.c.k_scales) + ph;
-  int8_t* codes = (which ? p.c.v : p.c.k) + ph * P * D;
-  const T* x = static_cast<const T*>(p.src[which]) + tok * p.ld[which] + (size_t)h * D;
+  const int held = pg == first ? (int)a - pg * P : 0;                   // earlier tokens of the sequence in this page
+  const int end = (int)::min(a + n - (long long)pg * P, (long long)P);  // new tokens: slots held .. end
+  const long long tok = t0 + ((long long)pg * P + held - a);            // stacked row of slot `held`
+  const T* x = static_cast<const T*>(p.src[which]) + tok * p.ld[which];
   const long long ld = p.ld[which];
-  const int vpr = D / 8, vecs = (end - held) * vpr;
-  auto load = [&](int i, float (&f)[8]) {
-    const T* r = x + (i / vpr) * ld + (i % vpr) * 8;
+  const int shift = D == 128 ? 4 : 3, vpr = 1 << shift, vecs = (end - held) << shift;
+  auto load = [&](int h, int i, float (&f)[8]) {
+    const T* r = x + (i >> shift) * ld + (size_t)h * D + (i & (vpr - 1)) * 8;
     if (VEC) {
       load8<DT>(r, f);
     } else {
@@ -93,41 +96,94 @@ __global__ void __launch_bounds__(THREADS) cache_write_kernel(WriteParams p) {
       for (int e = 0; e < 8; e++) f[e] = Elem<DT>::widen(r[e]);
     }
   };
-  float m = 0.0f;
-  for (int i = threadIdx.x; i < vecs; i += THREADS) {
-    float f[8];
-    load(i, f);
+  float f[NV][8];
+  auto fetch = [&](int h) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) m = fmaxf(m, finite_abs(f[e]));
+    for (int j = 0; j < NV; j++)
+      if ((int)threadIdx.x + j * THREADS < vecs) load(h, (int)threadIdx.x + j * THREADS, f[j]);
+  };
+  fetch(h0);  // on their way before the page's id is here
+  if (pid < 0 || pid >= p.c.n_pages) {
+    if (threadIdx.x == 0) atomicCAS(p.status + 1, 0, VXG_DEV_CACHE_INDEX);
+    return;
   }
+  float* scales = (which ? p.c.v_scales : p.c.k_scales) + (size_t)pid * H;
+  int8_t* pages = (which ? p.c.v : p.c.k) + (size_t)pid * H * P * D;
+  float s0 = held ? scales[h0] : 0.0f;
+  for (int h = h0; h < h1; h++) {
+    float m = 0.0f;
+    bool plain = true;  // every value of the thread finite
+    auto look = [&](const float (&v)[8]) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if ((threadIdx.x & 31) == 0) wmax[threadIdx.x >> 5] = m;
-  const float s0 = held ? *scale : 0.0f;
-  __syncthreads();  // every thread has read the old scale before one of them writes the new one
+      for (int e = 0; e < 8; e++) {
+        const float u = finite_abs(v[e]);
+        plain = plain && u == fabsf(v[e]);
+        m = fmaxf(m, u);
+      }
+    };
 #pragma unroll
-  for (int w = 0; w < THREADS / 32; w++) m = fmaxf(m, wmax[w]);
-  const float s1 = fmaxf(s0, m > 0.0f ? fmaxf(__fdiv_rn(m, 127.0f), 1.17549435e-38f) : 0.0f);
-  if (threadIdx.x == 0) *scale = s1;
-  if (held && s1 != s0) {
-    const float ratio = __fdiv_rn(s0, s1);
-    for (int i = threadIdx.x; i < held * D / 4; i += THREADS) {
-      const uint32_t w = reinterpret_cast<uint32_t*>(codes)[i];
-      uint32_t r = 0;
+    for (int j = 0; j < NV; j++)
+      if ((int)threadIdx.x + j * THREADS < vecs) look(f[j]);
+    if (LONG)
+      for (int i = threadIdx.x + NV * THREADS; i < vecs; i += THREADS) {
+        float g[8];
+        load(h, i, g);
+        look(g);
+      }
 #pragma unroll
-      for (int e = 0; e < 4; e++) r |= code8((float)(int8_t)(w >> (8 * e)), ratio) << (8 * e);
-      reinterpret_cast<uint32_t*>(codes)[i] = r;
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if ((threadIdx.x & 31) == 0) wmax[h & 1][threadIdx.x >> 5] = m;
+    __syncthreads();  // also: every thread has read the old scale before one of them writes the new one
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; w++) m = fmaxf(m, wmax[h & 1][w]);
+    const float s1 = fmaxf(s0, m > 0.0f ? fmaxf(__fdiv_rn(m, 127.0f), 1.17549435e-38f) : 0.0f);
+    int8_t* codes = pages + (size_t)h * P * D;
+    if (threadIdx.x == 0) scales[h] = s1;
+    if (held && s1 != s0) {
+      const float ratio = __fdiv_rn(s0, s1);
+      for (int i = threadIdx.x; i < held * D / 4; i += THREADS) {
+        const uint32_t w = reinterpret_cast<uint32_t*>(codes)[i];
+        uint32_t r = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) r |= code8((float)(int8_t)(w >> (8 * e)), ratio) << (8 * e);
+        reinterpret_cast<uint32_t*>(codes)[i] = r;
+      }
+    }
+    const float inv = s1 > 0.0f ? __fdiv_rn(1.0f, s1) : 0.0f;  // finite: s1 >= 2^-126
+    auto put = [&](int i, const float (&v)[8]) {
+      uint32_t w[2] = {0, 0};
+      if (plain) {  // |value * inv| <= 127 (1 + 2^-23): the code is the rounding shifter's low byte
+#pragma unroll
+        for (int k = 0; k < 2; k++) w[k] = quant_word_fast(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3], inv);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) w[e >> 2] |= code8(v[e], inv) << (8 * (e & 3));
+      }
+      *reinterpret_cast<uint2*>(codes + (size_t)held * D + (size_t)i * 8) = make_uint2(w[0], w[1]);
+    };
+#pragma unroll
+    for (int j = 0; j < NV; j++)
+      if ((int)threadIdx.x + j * THREADS < vecs) put((int)threadIdx.x + j * THREADS, f[j]);
+    if (LONG)
+      for (int i = threadIdx.x + NV * THREADS; i < vecs; i += THREADS) {
+        float g[8];
+        load(h, i, g);
+        put(i, g);
+      }
+    if (h + 1 < h1) {
+      fetch(h + 1);
+      s0 = held ? scales[h + 1] : 0.0f;
     }
   }
-  const float inv = s1 > 0.0f ? __fdiv_rn(1.0f, s1) : 0.0f;
-  for (int i = threadIdx.x; i < vecs; i += THREADS) {
-    float f[8];
-    load(i, f);
-    uint32_t w[2] = {0, 0};
-#pragma unroll
-    for (int e = 0; e < 8; e++) w[e >> 2] |= code8(f[e], inv) << (8 * (e & 3));
-    *reinterpret_cast<uint2*>(codes + (size_t)held * D + (size_t)i * 8) = make_uint2(w[0], w[1]);
-  }
+}
+
+template <int DT, int THREADS, int NV, bool LONG>
+void write_launch(WriteParams p, int items, bool vec, cudaStream_t st) {
+  // heads of a block: all of them once that leaves four blocks for every SM
+  p.run = (int)std::max(1LL, std::min((long long)p.c.heads, 2LL * items * p.c.heads / (4LL * sm_count())));
+  const dim3 grid((unsigned)items, (unsigned)((p.c.heads + p.run - 1) / p.run), 2);
+  if (vec) cache_write_kernel<DT, THREADS, NV, true, LONG><<<grid, THREADS, 0, st>>>(p);
+  else cache_write_kernel<DT, THREADS, NV, false, LONG><<<grid, THREADS, 0, st>>>(p);
 }
 
 struct ReadParams {
@@ -146,14 +202,11 @@ __global__ void __launch_bounds__(256) cache_read_kernel(ReadParams p) {
   using T = typename Elem<DT>::type;
   const int P = p.c.page, H = p.c.heads, D = p.c.head_dim, vpt = H * D / 16;
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  // the sequence of the warp's first token, then on to this thread's
+  int lo = find32(p.n_seq, (i & ~31LL) / vpt, [&](int s) { return (long long)__ldg(p.cu + s); });
   const long long tok = i / vpt;
   if (tok >= p.total) return;
-  int lo = 0, hi = p.n_seq;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (__ldg(p.cu + mid) <= tok) lo = mid;
-    else hi = mid;
-  }
+  while (lo + 1 < p.n_seq && __ldg(p.cu + lo + 1) <= tok) lo++;
   const long long a = __ldg(p.start + lo), at = tok - __ldg(p.cu + lo);
   if (at < 0 || tok >= __ldg(p.cu + lo + 1)) return;  // rows behind the last sequence stay as they are
   const int e = (int)(i % vpt) * 16, h = e / D;
@@ -238,12 +291,16 @@ vxg_status vxg_cache_write(const vxg_kv_cache* c, const void* k, long long ld_k,
   VXG_ARG(status, "no CUDA device");
   const long long eb = (long long)dtype_bytes(dtype);
   const bool vec = (((uintptr_t)k | (uintptr_t)v | (uintptr_t)(ld_k * eb) | (uintptr_t)(ld_v * eb)) & 15) == 0;
-  cache::WriteParams p = {*c, {k, v}, {ld_k, ld_v}, table, start, cu, status, total, n_seq, max_pages};
-  const dim3 grid((unsigned)items, (unsigned)c->heads, 2);
+  cache::WriteParams p = {*c, {k, v}, {ld_k, ld_v}, table, start, cu, status, total, n_seq, max_pages, 1};
   with_dtype(dtype, [&](auto tag) {
     constexpr int DT = decltype(tag)::value;
-    if (vec) cache::cache_write_kernel<DT, true><<<grid, cache::THREADS, 0, (cudaStream_t)stream>>>(p);
-    else cache::cache_write_kernel<DT, false><<<grid, cache::THREADS, 0, (cudaStream_t)stream>>>(p);
+    cudaStream_t st = (cudaStream_t)stream;
+    const int most = std::min(total, c->page) * c->head_dim / 8;  // vectors of a page and head
+    // a few tokens a sequence: small blocks, which all fit the GPU at once; measured, 64 sequences of one token: see above
+    if (total <= 4LL * n_seq) cache::write_launch<DT, 64, 1, true>(p, (int)items, vec, st);
+    else if (most <= 512) cache::write_launch<DT, 256, 2, false>(p, (int)items, vec, st);
+    else if (most <= 1024) cache::write_launch<DT, 256, 4, false>(p, (int)items, vec, st);
+    else cache::write_launch<DT, 256, 8, false>(p, (int)items, vec, st);
   });
   note_launch();
   VXG_CUDA(cudaGetLastError());
