@@ -87,8 +87,9 @@ __global__ void __launch_bounds__(THREADS) cache_write_kernel(const WriteParams 
   const T* x = static_cast<const T*>(p.src[which]) + tok * p.ld[which];
   const long long ld = p.ld[which];
   const int shift = D == 128 ? 4 : 3, vpr = 1 << shift, vecs = (end - held) << shift;
+  auto at = [&](int h, int i) { return x + (i >> shift) * ld + (size_t)h * D + (i & (vpr - 1)) * 8; };
   auto load = [&](int h, int i, float (&f)[8]) {
-    const T* r = x + (i >> shift) * ld + (size_t)h * D + (i & (vpr - 1)) * 8;
+    const T* r = at(h, i);
     if (VEC) {
       load8<DT>(r, f);
     } else {
@@ -96,13 +97,19 @@ __global__ void __launch_bounds__(THREADS) cache_write_kernel(const WriteParams 
       for (int e = 0; e < 8; e++) f[e] = Elem<DT>::widen(r[e]);
     }
   };
-  float f[NV][8];
-  auto fetch = [&](int h) {
+  // the thread's first HELD vectors stay in registers as they lie in memory
+  constexpr int HELD = VEC ? NV : 0;
+  Raw<DT> raw[NV], ahead[NV];
+  auto fetch = [&](int h, Raw<DT> (&v)[NV]) {
 #pragma unroll
-    for (int j = 0; j < NV; j++)
-      if ((int)threadIdx.x + j * THREADS < vecs) load(h, (int)threadIdx.x + j * THREADS, f[j]);
+    for (int j = 0; j < HELD; j++)
+      if ((int)threadIdx.x + j * THREADS < vecs) {
+        const uint4* r = reinterpret_cast<const uint4*>(at(h, (int)threadIdx.x + j * THREADS));
+        v[j].w[0] = r[0];
+        if constexpr (DT == VXG_DT_F32) v[j].w[1] = r[1];
+      }
   };
-  fetch(h0);  // on their way before the page's id is here
+  fetch(h0, raw);  // on their way before the page's id is here
   if (pid < 0 || pid >= p.c.n_pages) {
     if (threadIdx.x == 0) atomicCAS(p.status + 1, 0, VXG_DEV_CACHE_INDEX);
     return;
@@ -111,25 +118,39 @@ __global__ void __launch_bounds__(THREADS) cache_write_kernel(const WriteParams 
   int8_t* pages = (which ? p.c.v : p.c.k) + (size_t)pid * H * P * D;
   float s0 = held ? scales[h0] : 0.0f;
   for (int h = h0; h < h1; h++) {
-    float m = 0.0f;
-    bool plain = true;  // every value of the thread finite
-    auto look = [&](const float (&v)[8]) {
+    float s0n = 0.0f;
+    if (h + 1 < h1) {
+      fetch(h + 1, ahead);
+      if (held) s0n = scales[h + 1];
+    }
+    auto each = [&](auto&& f) {  // f(i, values) for the thread's vectors
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const float u = finite_abs(v[e]);
-        plain = plain && u == fabsf(v[e]);
-        m = fmaxf(m, u);
-      }
+      for (int j = 0; j < HELD; j++)
+        if ((int)threadIdx.x + j * THREADS < vecs) {
+          float v[8];
+          unpack<DT>(raw[j], v);
+          f((int)threadIdx.x + j * THREADS, v);
+        }
+      if (LONG || !VEC)
+        for (int i = threadIdx.x + HELD * THREADS; i < vecs; i += THREADS) {
+          float v[8];
+          load(h, i, v);
+          f(i, v);
+        }
     };
+    float m = 0.0f, seen = 0.0f;  // seen: NaN if one of the thread's values is
+    each([&](int, const float (&v)[8]) {
 #pragma unroll
-    for (int j = 0; j < NV; j++)
-      if ((int)threadIdx.x + j * THREADS < vecs) look(f[j]);
-    if (LONG)
-      for (int i = threadIdx.x + NV * THREADS; i < vecs; i += THREADS) {
-        float g[8];
-        load(h, i, g);
-        look(g);
-      }
+      for (int e = 0; e < 8; e++) m = fmaxf(m, fabsf(v[e])), seen = max_nan(seen, v[e]);
+    });
+    const bool plain = seen == seen && m <= 3.402823466e38f;  // every value of the thread finite
+    if (!plain) {
+      m = 0.0f;
+      each([&](int, const float (&v)[8]) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) m = fmaxf(m, finite_abs(v[e]));
+      });
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if ((threadIdx.x & 31) == 0) wmax[h & 1][threadIdx.x >> 5] = m;
@@ -150,7 +171,7 @@ __global__ void __launch_bounds__(THREADS) cache_write_kernel(const WriteParams 
       }
     }
     const float inv = s1 > 0.0f ? __fdiv_rn(1.0f, s1) : 0.0f;  // finite: s1 >= 2^-126
-    auto put = [&](int i, const float (&v)[8]) {
+    each([&](int i, const float (&v)[8]) {
       uint32_t w[2] = {0, 0};
       if (plain) {  // |value * inv| <= 127 (1 + 2^-23): the code is the rounding shifter's low byte
 #pragma unroll
@@ -160,20 +181,10 @@ __global__ void __launch_bounds__(THREADS) cache_write_kernel(const WriteParams 
         for (int e = 0; e < 8; e++) w[e >> 2] |= code8(v[e], inv) << (8 * (e & 3));
       }
       *reinterpret_cast<uint2*>(codes + (size_t)held * D + (size_t)i * 8) = make_uint2(w[0], w[1]);
-    };
+    });
+    s0 = s0n;
 #pragma unroll
-    for (int j = 0; j < NV; j++)
-      if ((int)threadIdx.x + j * THREADS < vecs) put((int)threadIdx.x + j * THREADS, f[j]);
-    if (LONG)
-      for (int i = threadIdx.x + NV * THREADS; i < vecs; i += THREADS) {
-        float g[8];
-        load(h, i, g);
-        put(i, g);
-      }
-    if (h + 1 < h1) {
-      fetch(h + 1);
-      s0 = held ? scales[h + 1] : 0.0f;
-    }
+    for (int j = 0; j < HELD; j++) raw[j] = ahead[j];
   }
 }
 

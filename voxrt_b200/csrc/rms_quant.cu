@@ -62,29 +62,6 @@ __device__ __forceinline__ float inv_root(double v) {
   return (float)fma(y * e, fma(e, 0.375, 0.5), y);
 }
 
-// Eight elements as they lie in memory.
-template <int DT>
-struct Raw {
-  uint4 w[DT == VXG_DT_F32 ? 2 : 1];
-};
-template <int DT>
-__device__ __forceinline__ void unpack(const Raw<DT>& r, float (&v)[8]) {
-  if constexpr (DT == VXG_DT_F32) {
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-      v[4 * i] = __uint_as_float(r.w[i].x), v[4 * i + 1] = __uint_as_float(r.w[i].y);
-      v[4 * i + 2] = __uint_as_float(r.w[i].z), v[4 * i + 3] = __uint_as_float(r.w[i].w);
-    }
-  } else {
-    const uint32_t w[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const float2 f = widen2<DT>(w[i]);
-      v[2 * i] = f.x, v[2 * i + 1] = f.y;
-    }
-  }
-}
-
 // NV vectors a thread, vector j of thread t covers elements 8 (t + j * threads) .. + 8. NORM: with the norm; else the
 // row is quantised as it is. A block works off rows blockIdx, blockIdx + gridDim, .. and asks for the next row's vectors
 // before the current one's reductions, whose barriers would else leave the memory idle. One element at a time (VEC
