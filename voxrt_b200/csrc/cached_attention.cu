@@ -6,10 +6,10 @@
 // Arithmetic. Codes are exact in f16, so both products run on mma.m16n8k16 with f16 operands and f32 sums. A query row
 // is scaled by a power of two so that its largest element lies in [2^14, 2^15): bf16 and f16 queries are then exact
 // down to 2^-29 of that element; f32 queries are split into two f16 parts (22 bits). The page's key scale, the row's
-// power of two, `scale` and log2(e) multiply the f32 sum. The softmax is kept in f32 with a running maximum and sum;
-// a probability enters the second product as f16(p * 2^14 * v_scale / ref), ref being the largest value scale met so
-// far (rounding 2^-11 of each term at most, 2^-39 absolute against the largest; two parts for f32), and ref and 2^-14 multiply
-// the result. (The kernels for few and many rows let the maximum lag by up to 2^8 and use 2^7 for 2^14.) The sum of the row is taken from the unrounded p.
+// power of two, `scale` and log2(e) multiply the f32 sum. The softmax is kept in f32 with a running sum and a reference
+// which may lag behind the maximum by up to 2^8, so that it seldom moves; a probability enters the second product as f16(p * 2^7 * v_scale /
+// ref), ref being the largest value scale met so far (rounding 2^-11 of each term at most, 2^-32 absolute against the
+// largest; two parts for f32), and ref and 2^-7 multiply the result. The sum of the row is taken from the unrounded p.
 //
 // Work split. A tile is MT consecutive (query, query head) rows of one sequence and KV head, so a key is read once for
 // all the query heads that share it. The keys it sees, in blocks of 64, times all tiles and KV heads form one line of
@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(THREADS, 2)
   using Lay = Layout<HD>;
   using T = typename Elem<DT>::type;
   constexpr bool SPLIT = DT == VXG_DT_F32;
-  constexpr int TOK = 64;  // keys of a block that one warp takes
+  constexpr int TOK = 32;  // keys a warp takes at a time
   constexpr bool BIASED = !SPLIT;
   constexpr int KS = HD / 16;         // k steps of the first product
   extern __shared__ uint8_t smem_raw[];
@@ -91,7 +91,8 @@ __global__ void __launch_bounds__(THREADS, 2)
 
   // -------------------------------------------------------------------------------------------------- consumers
   const int g = lane >> 2, c = lane & 3;
-  int it = 0;
+  int st = 0;
+  uint32_t phase = 0;
   bool ok = true;
   while (w.left > 0) {
     const Tile& t = w.t;
@@ -165,22 +166,16 @@ __global__ void __launch_bounds__(THREADS, 2)
 
     const int nb = t.nblk > 0 ? take : 0;
     float inv_ref = 0.0f;
-    for (int b = 0; b < nb; b++) {
-      const int st = (it + b) % Lay::STAGES;
-      if (ok && !wait_phase(full + st, ((it + b) / Lay::STAGES) & 1, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN)) ok = false;
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      const uint8_t* kt = smem + st * Lay::STAGE;
-      const uint8_t* vt = kt + Lay::TILE;
-      const int key0 = (t.blk0 + off + b) * BK;
-      constexpr int tok0 = 0;
+    // 32 keys of a block: what fits the registers beside O and Q
+    auto keys32 = [&](auto tag, const uint8_t* kt, const uint8_t* vt, const float* scales, int key0) {
+      constexpr bool masked = decltype(tag)::value;
       // ---- scores. 16-bit queries: the codes enter as 1152 + code, and the sums begin at -1152 times the row's sum
       float s[TOK / 8][4];
 #pragma unroll
       for (int j = 0; j < TOK / 8; j++) {
 #pragma unroll
         for (int k = 0; k < 4; k++) s[j][k] = BIASED ? bias[k >> 1] : 0.0f;
-        const int r = tok0 + 8 * j + g;
+        const int r = 8 * j + g;  // rows of 32 keys begin on a swizzle period
         uint32_t w[HD / 16];
         if (HD == 128) {
 #pragma unroll
@@ -200,55 +195,48 @@ __global__ void __launch_bounds__(THREADS, 2)
           if (SPLIT) mma_f16(s[j], qb[k], b0, b1);
         }
       }
-      // ---- scale, mask, running maximum
-      const bool inside = key0 >= all_lo && key0 + BK <= all_hi;
-      float mx[2] = {-INFINITY, -INFINITY};
+      // ---- scale, mask
+      float mx[2] = {-INFINITY, -INFINITY}, vsm = 0.0f;
 #pragma unroll
       for (int j = 0; j < TOK / 8; j++) {
-        const float ks = scales_s[st * 8 + (tok0 + 8 * j) / 16];
+        const float ks = scales[j / 2];
+        vsm = fmaxf(vsm, scales[4 + j / 2]);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
           float x = s[j][k] * (rowf[k >> 1] * ks);
-          if (!inside) {
-            const int key = key0 + tok0 + 8 * j + 2 * c + (k & 1);
+          if (masked) {
+            const int key = key0 + 8 * j + 2 * c + (k & 1);
             if (key < klo[k >> 1] || key >= khi[k >> 1]) x = -INFINITY;
           }
           s[j][k] = x;
           mx[k >> 1] = fmaxf(mx[k >> 1], x);
         }
       }
-      float vsm = 0.0f;
+      // ---- the rows' references move when a score has outgrown one by 2^8, ref when a value scale is larger than all before
+      const bool wider = vsm > S.ref;
+      if (__any_sync(0xffffffffu, wider || mx[0] > S.m[0] + 8.0f || mx[1] > S.m[1] + 8.0f)) {
+        float reff = 1.0f;
+        if (wider) {  // the same in the whole warp
+          reff = S.ref / vsm;
+          inv_ref = 128.0f / vsm;  // finite: a page's scale is 0 or at least 2^-126
+          S.ref = vsm;
+        }
 #pragma unroll
-      for (int j = 0; j < TOK / 16; j++) vsm = fmaxf(vsm, scales_s[st * 8 + 4 + tok0 / 16 + j]);
-      const float ref = fmaxf(S.ref, vsm);
-      float reff = 1.0f;
-      if (ref != S.ref) {  // the same in the whole warp
-        reff = S.ref / ref;
-        inv_ref = 1.0f / ref;  // finite: a page's scale is 0 or at least 2^-126
+        for (int e = 0; e < 2; e++) {
+          mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
+          mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
+          const float m = fmaxf(S.m[e], mx[e]), alpha = ex2(S.m[e] - (m == -INFINITY ? 0.0f : m));
+          S.m[e] = m;
+          S.l[e] *= alpha;
+#pragma unroll
+          for (int j = 0; j < HD / 8; j++) S.o[j][2 * e] *= alpha * reff, S.o[j][2 * e + 1] *= alpha * reff;
+        }
       }
-      float alpha[2], mu[2];
-#pragma unroll
-      for (int e = 0; e < 2; e++) {
-        mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
-        mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
-        const float m = fmaxf(S.m[e], mx[e]);
-        mu[e] = m == -INFINITY ? 0.0f : m;
-        alpha[e] = ex2(S.m[e] - mu[e]);
-        S.m[e] = m;
-        S.l[e] *= alpha[e];
-        alpha[e] *= reff;
-      }
-      S.ref = ref;
-      if (!__all_sync(0xffffffffu, alpha[0] == 1.0f && alpha[1] == 1.0f)) {
-#pragma unroll
-        for (int j = 0; j < HD / 8; j++)
-#pragma unroll
-          for (int k = 0; k < 4; k++) S.o[j][k] *= alpha[k >> 1];
-      }
-      // ---- probabilities and the second product, 16 keys a step
+      const float mu[2] = {S.m[0] == -INFINITY ? 0.0f : S.m[0], S.m[1] == -INFINITY ? 0.0f : S.m[1]};
+      // ---- probabilities, times 2^7 and the value scale, and the second product, 16 keys a step
 #pragma unroll
       for (int kk = 0; kk < TOK / 16; kk++) {
-        const float vf = scales_s[st * 8 + 4 + tok0 / 16 + kk] * inv_ref * 16384.0f;
+        const float vf = scales[4 + kk] * inv_ref;
         uint32_t pa[4], pb[4];
 #pragma unroll
         for (int e = 0; e < 2; e++)  // key group 2 kk + e
@@ -259,12 +247,11 @@ __global__ void __launch_bounds__(THREADS, 2)
             pa[2 * e + r] = pack_f16(p0 * vf, p1 * vf);
             if (SPLIT) pb[2 * e + r] = pack_rest(p0 * vf, p1 * vf, pa[2 * e + r]);
           }
-        const int r0 = tok0 + 16 * kk + 2 * c;
         constexpr int W = HD / 32;  // words of a key that a thread takes
         uint32_t x[4][W];
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-          const int r = r0 + (k & 1) + 8 * (k >> 1);
+          const int r = 16 * kk + 2 * c + (k & 1) + 8 * (k >> 1);
           if (HD == 128) {
             const uint4 y = *reinterpret_cast<const uint4*>(vt + r * 128 + ((g ^ (r & 7)) << 4));
             x[k][0] = y.x, x[k][1] = y.y, x[k][W - 2] = y.z, x[k][W - 1] = y.w;
@@ -284,17 +271,30 @@ __global__ void __launch_bounds__(THREADS, 2)
             if (SPLIT) mma_f16(S.o[4 * w + k], pb, b0, b1);
           }
       }
+    };
+    for (int b = 0; b < nb; b++) {
+      ok = __all_sync(0xffffffffu, wait_phase(full + st, phase, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN));
+      if (!ok) break;
+      const uint8_t* kt = smem + st * Lay::STAGE;
+      const int key0 = (t.blk0 + off + b) * BK;
+      const bool inside = key0 >= all_lo && key0 + BK <= all_hi;
+#pragma unroll 1
+      for (int k = 0; k < BK; k += TOK) {
+        const float* sc = scales_s + st * 8 + k / 16;
+        if (inside) keys32(std::false_type(), kt + k * HD, kt + Lay::TILE + k * HD, sc, key0 + k);
+        else keys32(std::true_type(), kt + k * HD, kt + Lay::TILE + k * HD, sc, key0 + k);
+      }
       __syncwarp();
       if (lane == 0) mbar_arrive(empty + st);
+      if (++st == Lay::STAGES) st = 0, phase ^= 1;
     }
-    it += nb;
     if (!ok) return;
 #pragma unroll
     for (int e = 0; e < 2; e++) {
       S.l[e] += __shfl_xor_sync(0xffffffffu, S.l[e], 1);
       S.l[e] += __shfl_xor_sync(0xffffffffu, S.l[e], 2);
     }
-    const float unit = S.ref * (1.0f / 16384.0f);
+    const float unit = S.ref * (1.0f / 128.0f);
     const bool whole = off == 0 && take == t.cost;
     float* part = p.part + ((size_t)blockIdx.x * MAX_PIECES + (w.first ? 0 : 1)) * MT * (HD + 2);
     // thread (g, c)'s columns: HD / 4 consecutive ones, the first HD / 8 in o[.][0 or 2], the rest in o[.][1 or 3]

@@ -164,10 +164,14 @@ cudaMemPool_t scratch_pool() {
 }
 
 int sm_count() {
+  static std::atomic<int> known[64];  // per device
   int dev = 0, n = 0;
-  cudaGetDevice(&dev);
+  if (cudaGetDevice(&dev) != cudaSuccess) return 1;
+  if (dev >= 0 && dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
   cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  return n > 0 ? n : 1;
+  if (n <= 0) return 1;
+  if (dev >= 0 && dev < 64) known[dev].store(n, std::memory_order_relaxed);
+  return n;
 }
 
 }  // namespace vxg

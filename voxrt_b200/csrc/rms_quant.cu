@@ -277,8 +277,9 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const int8_t* __restric
 // As many blocks as the GPU holds at once, or as there are rows.
 template <class Kernel>
 void start(Kernel k, const Params& p, dim3 grid, dim3 block, size_t smem, cudaStream_t st) {
-  int per_sm = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, (int)(block.x * block.y), smem) != cudaSuccess || per_sm < 1)
+  int per_sm = 1;
+  if (grid.x > (unsigned)sm_count() &&
+      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, (int)(block.x * block.y), smem) != cudaSuccess || per_sm < 1)
     per_sm = 1;
   grid.x = std::min(grid.x, (unsigned)(sm_count() * per_sm));
   k<<<grid, block, smem, st>>>(p);
