@@ -45,6 +45,7 @@ class KvCache:
         self.n_pages, self.heads, self.page, self.head_dim = k.shape
         self._desc = _Desc(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), *k.shape)
         self._ref = C.addressof(self._desc)
+        self._ws_bytes = {}  # attend's workspace size by its shape
 
     @classmethod
     def empty(cls, n_pages: int, heads: int, head_dim: int, page: int = 64, device=None) -> "KvCache":
@@ -100,7 +101,7 @@ class KvCache:
         lengths - n + i; it sees positions up to its own (causal) and, with window > 0, the last `window` of them. heads
         is a multiple of the cache's; neighbouring query heads share a cache head. scale defaults to head_dim ** -0.5."""
         idx, n_seq, width = self._batch(table, lengths, cu, stream, q, out)
-        if torch.cuda.current_device() != idx:  # the workspace's size is the current device's
+        if torch._C._cuda_getDevice() != idx:  # the workspace's size is the current device's
             with torch.cuda.device(idx):
                 return self.attend(q, table, lengths, cu, scale, causal, window, out, stream)
         heads, hd = q.shape[1] if q.dim() == 3 else 0, self.head_dim
@@ -114,7 +115,11 @@ class KvCache:
         ld_out = _stacked(out, heads, hd, "out")
         total = q.shape[0]
         # the workspace is this call's own: captured graphs and streams never share one
-        nb = lib().vxg_cache_attention_workspace_bytes(total, n_seq, heads, self.heads, hd, dt)
+        nb = self._ws_bytes.get((total, n_seq, heads, dt))
+        if nb is None:
+            nb = lib().vxg_cache_attention_workspace_bytes(total, n_seq, heads, self.heads, hd, dt)
+            if len(self._ws_bytes) < 4096:
+                self._ws_bytes[total, n_seq, heads, dt] = nb
         ws = _like(q, (nb,), torch.uint8, stream)
         _call(lib().vxg_cache_attention, idx, stream, (q, table, lengths, cu, out, self.k, self.v, self.ks, self.vs),
               self._ref, q.data_ptr(), ld_q, heads, dt, total, table.data_ptr(), n_seq, width, lengths.data_ptr(),

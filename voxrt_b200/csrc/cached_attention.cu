@@ -7,17 +7,18 @@
 // is scaled by a power of two so that its largest element lies in [2^14, 2^15): bf16 and f16 queries are then exact
 // down to 2^-29 of that element; f32 queries are split into two f16 parts (22 bits). The page's key scale, the row's
 // power of two, `scale` and log2(e) multiply the f32 sum. The softmax is kept in f32 with a running sum and a reference
-// which may lag behind the maximum by up to 2^8, so that it seldom moves; a probability enters the second product as f16(p * 2^7 * v_scale /
-// ref), ref being the largest value scale met so far (rounding 2^-11 of each term at most, 2^-32 absolute against the
-// largest; two parts for f32), and ref and 2^-7 multiply the result. The sum of the row is taken from the unrounded p.
+// that may lag behind the maximum by up to 2^8, so that it seldom moves; a probability enters the second product as
+// f16(p * 2^7 * v_scale / ref), ref being the largest value scale met so far (rounding 2^-11 of each term at most, 2^-32
+// absolute against the largest; two parts for f32), and ref and 2^-7 multiply the result. The sum of the row is taken
+// from the unrounded p.
 //
 // Work split. A tile is MT consecutive (query, query head) rows of one sequence and KV head, so a key is read once for
 // all the query heads that share it. The keys it sees, in blocks of 64, times all tiles and KV heads form one line of
 // work units that is cut into equal shares, one a CTA: a CTA works off its share tile by tile, and a tile that spans
 // shares leaves partial results (maximum, sum, unnormalised row) that a second small kernel joins. Lengths are read on
 // the device, so the launch does not depend on them and can be captured; every CTA finds its share with one scan.
-// This file: tiles of 64 rows, a consumer warp takes 16 rows and all 64 keys of a block. cached_attention_few.cu: up to 16
-// rows. cached_attention_tc.cu: 256 rows.
+// This file: tiles of 64 rows, a consumer warp takes 16 rows and all 64 keys of a block (f32 queries, heads of 64).
+// cached_attention_few.cu: up to 16 rows. cached_attention_tc.cu: 256 rows.
 // A fifth warp brings the codes by TMA (one box per page, 128- or 64-byte swizzle so that the operand reads below are
 // free of bank conflicts) and the scales into a ring of stages. Operand layout: the k slots of a step are permuted so
 // that a thread's operand words are consecutive codes (keys: of one key; values: one word of four keys, transposed by
@@ -70,7 +71,6 @@ __global__ void __launch_bounds__(THREADS, 2)
   uint64_t* empty = full + Lay::STAGES;
   __shared__ Piece first_s;  // the share's first piece
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int KV = p.c.heads, PL = p.page_log2, P = 1 << PL;  // pages are powers of two
 
   if (tid == 0) {
     for (int i = 0; i < Lay::STAGES; i++) {
@@ -332,11 +332,15 @@ __global__ void __launch_bounds__(THREADS, 2)
 
 constexpr int CTAS_PER_SM = 2;
 
-// The kernels by the average number of (query, query head) rows a sequence and KV head has: up to 8 and 16 rows, tiles
-// of as many; up to 96, tiles of 64; beyond, tiles of 256 on tcgen05 (16-bit queries).
+// The kernels by the average number of (query, query head) rows a sequence and KV head has. Up to 8 and 16 rows: tiles of
+// as many. More: tiles of 256 on tcgen05, which pay from a handful of rows on although most of a tile is empty then
+// (measured, 16 sequences over 4000 tokens, heads of 128: 20 rows 97 us against 124 with tiles of 64, 96 rows 110 against
+// 232); but tiles of 64 for f32 queries, whose two parts would not fit a 256-row tile, and for up to 64 rows of heads of
+// 64, where they are the faster ones (8 sequences over 1000, 32 rows: 30 us against 34).
 static vxg_status plan(int total, int n_seq, int heads, int kv, int hd, int dtype, Plan* pl) {
   const long long share = heads / kv, rows = (long long)total * share;
-  pl->mt = rows <= 8LL * n_seq ? 8 : rows <= 16LL * n_seq ? 16 : rows <= 96LL * n_seq || dtype == VXG_DT_F32 ? 64 : 256;
+  const bool tiles64 = dtype == VXG_DT_F32 || (hd == 64 && rows <= 64LL * n_seq);
+  pl->mt = rows <= 8LL * n_seq ? 8 : rows <= 16LL * n_seq ? 16 : tiles64 ? 64 : 256;
   const long long slots = rows / pl->mt + n_seq;
   if (slots > 0x3FFFFFFF) {
     set_error("%d rows of %d heads are more than one launch covers", total, heads);
@@ -415,7 +419,11 @@ vxg_status vxg_cache_attention(const vxg_kv_cache* c, const void* q, long long l
   if (pl.mt <= 16) return catt::launch_few(p, pl, c->head_dim, dtype, st);
   with_dtype(dtype, [&](auto tag) {
     constexpr int DT = decltype(tag)::value;
-    r = c->head_dim == 128 ? catt::launch<128, DT>(p, pl, st) : catt::launch<64, DT>(p, pl, st);
+    if constexpr (DT == VXG_DT_F32) {
+      r = c->head_dim == 128 ? catt::launch<128, DT>(p, pl, st) : catt::launch<64, DT>(p, pl, st);
+    } else {
+      r = catt::launch<64, DT>(p, pl, st);
+    }
   });
   return r;
 }

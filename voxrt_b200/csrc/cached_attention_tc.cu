@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     // descriptor = fixed upper word, lower word = address / 16 and the offset between 64-column halves
     const uint64_t desc_k = umma_desc_sw128(smem_u32(smem)), desc_mn = umma_desc_sw128_mn(smem_u32(smem), Lay::HALF);
     bool ok = true;
-    uint32_t nq = 0, np = 0;  // pieces begun, probabilities consumed (per half)
+    uint32_t nq0 = 0, nq1 = 0, np0 = 0, np1 = 0;  // by half: pieces begun, probabilities consumed
     int it = 0;
     auto wait = [&](uint64_t* b, uint32_t phase) {
       if (ok && !wait_phase(b, phase & 1, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN)) ok = false;
@@ -302,27 +302,35 @@ __global__ void __launch_bounds__(THREADS, 1)
       __syncwarp();
     };
     for (Blocks x(p, first); !x.done() && ok;) {
-      if (!wait(qfull, nq) || !wait(kfull + (it & 1), it >> 1)) break;
+      const bool two = x.w.t.rows > 128;  // else the second half has no rows and stays out
+      if (!wait(qfull, nq0) || !wait(kfull + (it & 1), it >> 1)) break;
       scores(0, it & 1);
-      if (!wait(qfull + 1, nq)) break;
-      scores(1, it & 1);
+      nq0++;
+      if (two) {
+        if (!wait(qfull + 1, nq1)) break;
+        scores(1, it & 1);
+        nq1++;
+      }
       commit(kempty + (it & 1));
-      nq++;
       const int nb = x.nb;
-      for (int b = 0; b < nb; b++, it++, np++) {
+      for (int b = 0; b < nb; b++, it++) {
         const bool more = b + 1 < nb;
         const int st = it & 1, sn = st ^ 1;
-        if (!wait(vfull + st, it >> 1) || !wait(pfull, np)) break;
+        if (!wait(vfull + st, it >> 1) || !wait(pfull, np0)) break;
+        np0++;
         values(0, st, b == 0, !more);
         if (more) {
           if (!wait(kfull + sn, (it + 1) >> 1)) break;
           scores(0, sn);
         }
-        if (!wait(pfull + 1, np)) break;
-        values(1, st, b == 0, !more);
+        if (two) {
+          if (!wait(pfull + 1, np1)) break;
+          np1++;
+          values(1, st, b == 0, !more);
+        }
         commit(vempty + st);
         if (more) {
-          scores(1, sn);
+          if (two) scores(1, sn);
           commit(kempty + sn);
         }
         x.next(p);
@@ -338,9 +346,14 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t lanes = (uint32_t)wrow << 16;
     const uint32_t S = tmem + lanes + half * 128, O = tmem + lanes + 256 + half * HD;
     bool ok = true;
-    uint32_t it = 0, pieces = 0;
+    // blocks and pieces with keys so far: of this half (its barriers), of all halves (the rings)
+    uint32_t it = 0, pieces = 0, ring = 0, ring_piece = 0;
     for (Piece w = first; w.left > 0 && ok; w.next(p, MT, BK)) {
       const Tile& t = w.t;
+      if (half * 128 >= t.rows) {
+        if (t.nblk > 0) ring += w.take(), ring_piece++;
+        continue;
+      }
       const int take = w.take(), nb = t.nblk > 0 ? take : 0;
       const bool live = r < t.rows;
       const int rr = t.r0 + (live ? r : 0), i = rr / p.share, head = w.h * p.share + rr % p.share;
@@ -397,15 +410,15 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int all_hi = __reduce_min_sync(0xffffffffu, live ? khi : 0x7FFFFFFF);
         const int all_lo = __reduce_max_sync(0xffffffffu, live ? klo : 0);
 
-        for (int b = 0; b < nb; b++, it++) {
+        for (int b = 0; b < nb; b++, it++, ring++) {
           if (ok && !wait_phase(sfull + half, it & 1, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN)) ok = false;
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
           const int key0 = (t.blk0 + w.off + b) * BK;
           const bool inside = key0 >= all_lo && key0 + BK <= all_hi;
-          const float* ks = ks_s + (it % RING) * 8;
-          if (b == 0) unit = ref_s[pieces % RING] * (1.0f / 256.0f);
+          const float* ks = ks_s + (ring % RING) * 8;
+          if (b == 0) unit = ref_s[ring_piece % RING] * (1.0f / 256.0f);
           // ---- the block's maximum
           float mx = -INFINITY;
           auto maximum = [&](auto tag) {
@@ -506,7 +519,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
-        pieces++;
+        pieces++, ring_piece++;
       }
       // ---- the row's result, whole or for the join
       const bool whole = w.off == 0 && take == t.cost;

@@ -97,7 +97,7 @@ def _call(fn, idx: int, stream, used, *args):
         for t in used:
             if t is not None:
                 t.record_stream(stream)
-    if torch.cuda.current_device() == idx:
+    if torch._C._cuda_getDevice() == idx:
         status = fn(*args, raw)
     else:
         with torch.cuda.device(idx):
