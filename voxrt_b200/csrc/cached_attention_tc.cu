@@ -19,7 +19,7 @@ namespace vxg {
 namespace catt {
 namespace tc {
 
-constexpr int MT = 256, BK = 128;
+constexpr int MT = 256, BK = 128, SB = 64;  // rows, keys of an operand stage, keys of a step of the softmax
 constexpr int SOFT_WARPS = 8, CONV_WARPS = 4, MMA_WARP = SOFT_WARPS + CONV_WARPS, LOAD_WARP = MMA_WARP + 1;
 constexpr int THREADS = (LOAD_WARP + 1) * 32;
 // Blocks' scales and pieces' refs in flight: the loading warp fills block j only after block j - 1 has found a free operand
@@ -39,7 +39,7 @@ struct Layout {
   static constexpr uint32_t VF = KS + RING * 32;          // [RING][8] f32: their value scales / ref * 2^8
   static constexpr uint32_t REF = VF + RING * 32;         // [RING] f32
   static constexpr uint32_t BARS = REF + RING * 4;
-  static constexpr uint32_t BYTES = BARS + 21 * 8 + 1024;
+  static constexpr uint32_t BYTES = BARS + 25 * 8 + 1024;
   static_assert(BYTES <= 232448, "shared memory budget");
 };
 
@@ -81,9 +81,9 @@ __global__ void __launch_bounds__(THREADS, 1)
   float* ref_s = reinterpret_cast<float*>(smem + Lay::REF);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Lay::BARS);
   uint64_t *kfull = bars, *kempty = bars + 2, *vfull = bars + 4, *vempty = bars + 6;  // by stage
-  uint64_t *qfull = bars + 8, *sfull = bars + 10, *pfull = bars + 12, *ofull = bars + 14;  // by half
-  uint64_t* drain = bars + 16;
-  uint64_t *rkfull = bars + 17, *rkempty = bars + 18, *rvfull = bars + 19, *rvempty = bars + 20;
+  uint64_t *qfull = bars + 8, *sfull = bars + 10, *pfull = bars + 14, *odone = bars + 18;  // by half; sfull, pfull: and buffer
+  uint64_t* drain = bars + 20;
+  uint64_t *rkfull = bars + 21, *rkempty = bars + 22, *rvfull = bars + 23, *rvempty = bars + 24;
   __shared__ Piece first_s;
   __shared__ uint32_t holder;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -96,9 +96,11 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(vfull + i, CONV_WARPS);
       mbar_init(vempty + i, 1);
       mbar_init(qfull + i, 4);
+      mbar_init(odone + i, 1);
+    }
+    for (int i = 0; i < 4; i++) {
       mbar_init(sfull + i, 1);
       mbar_init(pfull + i, 4);
-      mbar_init(ofull + i, 1);
     }
     mbar_init(drain, 1);
     mbar_init(rkfull, 1);
@@ -261,12 +263,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     // --------------------------------------------------------------------------------------------- MMA issuer
     // The whole warp walks and waits, so that the operand descriptors stay in uniform registers, and one lane issues.
     // With one lane doing all of it, the descriptors' arithmetic took longer than the products.
-    constexpr uint32_t QK = idesc_f16(128, BK, false), PV = idesc_f16(128, HD, true);
+    constexpr uint32_t QK = idesc_f16(128, SB, false), PV = idesc_f16(128, HD, true);
     const bool leader = elect_one();
     // descriptor = fixed upper word, lower word = address / 16 and the offset between 64-column halves
     const uint64_t desc_k = umma_desc_sw128(smem_u32(smem)), desc_mn = umma_desc_sw128_mn(smem_u32(smem), Lay::HALF);
     bool ok = true;
-    uint32_t nq0 = 0, nq1 = 0, np0 = 0, np1 = 0;  // by half: pieces begun, probabilities consumed
+    uint32_t nq0 = 0, nq1 = 0, n0 = 0, n1 = 0;  // by half: pieces begun, steps whose values are under way
     int it = 0;
     auto wait = [&](uint64_t* b, uint32_t phase) {
       if (ok && !wait_phase(b, phase & 1, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN)) ok = false;
@@ -274,26 +276,27 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (ok) tc_fence_after();
       return ok;
     };
-    auto scores = [&](int half, int st) {
-      const uint64_t q = desc_k + (Lay::Q + half * Lay::OPER) / 16, k = desc_k + (Lay::K + st * Lay::OPER) / 16;
+    // step n of a half: 64 keys (`sub` of the operand stage), scores in buffer n % 2
+    auto scores = [&](int half, uint32_t n, int st, int sub) {
+      const uint32_t buf = n & 1, d = tmem + half * 128 + buf * SB;
+      const uint64_t q = desc_k + (Lay::Q + half * Lay::OPER) / 16, k = desc_k + (Lay::K + st * Lay::OPER + sub * SB * 128) / 16;
       if (leader) {
 #pragma unroll
         for (int c = 0; c < HD / 64; c++)
 #pragma unroll
           for (int j = 0; j < 4; j++)
-            mma_f16_ss(tmem + half * 128, q + c * (Lay::HALF / 16) + 2 * j, k + c * (Lay::HALF / 16) + 2 * j, QK,
-                       (c | j) != 0 ? 1u : 0u);
-        mma_commit(sfull + half);
+            mma_f16_ss(d, q + c * (Lay::HALF / 16) + 2 * j, k + c * (Lay::HALF / 16) + 2 * j, QK, (c | j) != 0 ? 1u : 0u);
+        mma_commit(sfull + 2 * half + buf);
       }
       __syncwarp();
     };
-    auto values = [&](int half, int st, bool fresh, bool last) {
-      const uint64_t v = desc_mn + (Lay::V + st * Lay::OPER) / 16;
+    auto values = [&](int half, uint32_t n, int st, int sub, bool fresh) {
+      const uint64_t v = desc_mn + (Lay::V + st * Lay::OPER + sub * SB * 128) / 16;
       if (leader) {
 #pragma unroll
-        for (int j = 0; j < BK / 16; j++)
-          mma_f16_ts(tmem + 256 + half * HD, tmem + half * 128 + 8 * j, v + j * 128, PV, fresh && j == 0 ? 0u : 1u);
-        if (last) mma_commit(ofull + half);
+        for (int j = 0; j < SB / 16; j++)
+          mma_f16_ts(tmem + 256 + half * HD, tmem + half * 128 + (n & 1) * SB + 8 * j, v + j * 128, PV, fresh && j == 0 ? 0u : 1u);
+        mma_commit(odone + half);
       }
       __syncwarp();
     };
@@ -303,37 +306,39 @@ __global__ void __launch_bounds__(THREADS, 1)
     };
     for (Blocks x(p, first); !x.done() && ok;) {
       const bool two = x.w.t.rows > 128;  // else the second half has no rows and stays out
+      const int nb = x.nb, ns = 2 * nb;
       if (!wait(qfull, nq0) || !wait(kfull + (it & 1), it >> 1)) break;
-      scores(0, it & 1);
+      for (int i = 0; i < 2; i++) scores(0, n0 + i, it & 1, i);
       nq0++;
       if (two) {
         if (!wait(qfull + 1, nq1)) break;
-        scores(1, it & 1);
+        for (int i = 0; i < 2; i++) scores(1, n1 + i, it & 1, i);
         nq1++;
       }
       commit(kempty + (it & 1));
-      const int nb = x.nb;
-      for (int b = 0; b < nb; b++, it++) {
-        const bool more = b + 1 < nb;
-        const int st = it & 1, sn = st ^ 1;
-        if (!wait(vfull + st, it >> 1) || !wait(pfull, np0)) break;
-        np0++;
-        values(0, st, b == 0, !more);
-        if (more) {
-          if (!wait(kfull + sn, (it + 1) >> 1)) break;
-          scores(0, sn);
+      for (int i = 0; i < ns; i++) {
+        const int st = it & 1, sub = i & 1;
+        const bool more = i + 2 < ns;
+        if (sub == 0 && !wait(vfull + st, it >> 1)) break;
+        if (!wait(pfull + (n0 & 1), n0 >> 1)) break;
+        values(0, n0, st, sub, i == 0);
+        if (more) {  // the step after next, over the probabilities that these products read
+          if (sub == 0 && !wait(kfull + (st ^ 1), (it + 1) >> 1)) break;
+          scores(0, n0 + 2, st ^ 1, sub);
         }
+        n0++;
         if (two) {
-          if (!wait(pfull + 1, np1)) break;
-          np1++;
-          values(1, st, b == 0, !more);
+          if (!wait(pfull + 2 + (n1 & 1), n1 >> 1)) break;
+          values(1, n1, st, sub, i == 0);
+          if (more) scores(1, n1 + 2, st ^ 1, sub);
+          n1++;
         }
-        commit(vempty + st);
-        if (more) {
-          if (two) scores(1, sn);
-          commit(kempty + sn);
+        if (sub == 1) {
+          commit(vempty + st);
+          if (more) commit(kempty + (st ^ 1));
+          it++;
+          x.next(p);
         }
-        x.next(p);
       }
     }
     commit(drain);  // nothing is in flight when the block ends
@@ -344,10 +349,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     constexpr int LPR = HD / 8, RPI = 32 / LPR;  // lanes a row and rows an access where a warp moves rows as wholes
     const int wrow = (warp & 3) * 32;            // the warp's first row of its half
     const uint32_t lanes = (uint32_t)wrow << 16;
-    const uint32_t S = tmem + lanes + half * 128, O = tmem + lanes + 256 + half * HD;
+    const uint32_t S0 = tmem + lanes + half * 128, O = tmem + lanes + 256 + half * HD;
     bool ok = true;
-    // blocks and pieces with keys so far: of this half (its barriers), of all halves (the rings)
-    uint32_t it = 0, pieces = 0, ring = 0, ring_piece = 0;
+    uint32_t it = 0;                     // steps of this half so far
+    uint32_t ring = 0, ring_piece = 0;   // blocks and pieces with keys of the CTA so far
     for (Piece w = first; w.left > 0 && ok; w.next(p, MT, BK)) {
       const Tile& t = w.t;
       if (half * 128 >= t.rows) {
@@ -410,43 +415,41 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int all_hi = __reduce_min_sync(0xffffffffu, live ? khi : 0x7FFFFFFF);
         const int all_lo = __reduce_max_sync(0xffffffffu, live ? klo : 0);
 
-        for (int b = 0; b < nb; b++, it++, ring++) {
-          if (ok && !wait_phase(sfull + half, it & 1, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN)) ok = false;
+        for (int b = 0; b < 2 * nb; b++, it++) {
+          const uint32_t buf = it & 1, S = S0 + buf * SB;
+          if (ok && !wait_phase(sfull + 2 * half + buf, (it >> 1) & 1, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN)) ok = false;
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
-          const int key0 = (t.blk0 + w.off + b) * BK;
-          const bool inside = key0 >= all_lo && key0 + BK <= all_hi;
-          const float* ks = ks_s + (ring % RING) * 8;
+          const int key0 = (t.blk0 + w.off) * BK + b * SB;
+          const bool inside = key0 >= all_lo && key0 + SB <= all_hi;
+          const float* ks = ks_s + ((ring + b / 2) % RING) * 8 + (b & 1) * (SB / 16);
           if (b == 0) unit = ref_s[ring_piece % RING] * (1.0f / 256.0f);
-          // ---- the block's maximum
+          // ---- the step's maximum
           float mx = -INFINITY;
           auto maximum = [&](auto tag) {
             constexpr bool masked = decltype(tag)::value;
-#pragma unroll 1
-            for (int c = 0; c < BK; c += 64) {
-              uint32_t a[2][32];
-              tmem_ld32(S + c, a[0]);
-              tmem_ld32(S + c + 32, a[1]);
-              tmem_wait_ld();
+            uint32_t a[2][32];
+            tmem_ld32(S, a[0]);
+            tmem_ld32(S + 32, a[1]);
+            tmem_wait_ld();
 #pragma unroll
-              for (int g = 0; g < 4; g++) {
-                const uint32_t* v = a[g >> 1] + 16 * (g & 1);
-                float y[16];
+            for (int g = 0; g < 4; g++) {
+              const uint32_t* v = a[g >> 1] + 16 * (g & 1);
+              float y[16];
 #pragma unroll
-                for (int j = 0; j < 16; j++) {
-                  y[j] = __uint_as_float(v[j]);
-                  const int key = key0 + c + 16 * g + j;
-                  if (masked && (key < klo || key >= khi)) y[j] = -INFINITY;
-                }
-                float x = max3(y[0], y[1], y[2]), z = max3(y[3], y[4], y[5]);
-                x = max3(x, y[6], y[7]), z = max3(z, y[8], y[9]);
-                x = max3(x, y[10], y[11]), z = max3(z, y[12], y[13]);
-                x = max3(x, y[14], y[15]), x = fmaxf(x, z);
-                // -inf x 0 would be NaN: a piece without a visible key has no maximum
-                const float f = rowf * ks[c / 16 + g];
-                mx = fmaxf(mx, masked && x == -INFINITY ? x : x * f);
+              for (int j = 0; j < 16; j++) {
+                y[j] = __uint_as_float(v[j]);
+                const int key = key0 + 16 * g + j;
+                if (masked && (key < klo || key >= khi)) y[j] = -INFINITY;
               }
+              float x = max3(y[0], y[1], y[2]), z = max3(y[3], y[4], y[5]);
+              x = max3(x, y[6], y[7]), z = max3(z, y[8], y[9]);
+              x = max3(x, y[10], y[11]), z = max3(z, y[12], y[13]);
+              x = max3(x, y[14], y[15]), x = fmaxf(x, z);
+              // -inf x 0 would be NaN: a piece without a visible key has no maximum
+              const float f = rowf * ks[g];
+              mx = fmaxf(mx, masked && x == -INFINITY ? x : x * f);
             }
           };
           if (inside) maximum(std::false_type());
@@ -457,7 +460,11 @@ __global__ void __launch_bounds__(THREADS, 1)
             const float alpha = grow ? ex2(m - mx) : 1.0f;
             if (grow) m = mx;
             l *= alpha;
-            if (b > 0) {
+            if (b > 0) {  // once the products of the step before are in O (those before them are, or these scores were not)
+              if (!wait_phase(odone + half, (it - 1) & 1, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN)) ok = false;
+              ok = __all_sync(0xffffffffu, ok);
+              if (!ok) break;
+              tc_fence_after();
 #pragma unroll 1
               for (int c = 0; c < HD; c += 32) {
                 uint32_t a[32];
@@ -470,15 +477,15 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
           }
           const float mm = m == -INFINITY ? 0.0f : m - 7.0f;  // probabilities times 2^7
-          // ---- probabilities over the scores: chunk c's 32 scores are read before its 16 columns are written
-          uint64_t sum[4] = {0, 0, 0, 0};  // eight partial sums of the block
+          // ---- probabilities over the scores: 32 scores are read before their 16 columns are written
+          uint64_t sum[4] = {0, 0, 0, 0};  // eight partial sums of the step
           auto exponentials = [&](auto tag) {
             constexpr bool masked = decltype(tag)::value;
             const uint64_t mm2 = pk2(-mm, -mm);
             uint32_t a[32];
             tmem_ld32(S, a);
 #pragma unroll 1
-            for (int c = 0; c < BK; c += 32) {
+            for (int c = 0; c < SB; c += 32) {
               uint64_t x[16];
               const float f0 = rowf * ks[c / 16], f1 = rowf * ks[c / 16 + 1];
               tmem_wait_ld();
@@ -487,7 +494,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 const float f = j < 8 ? f0 : f1;
                 x[j] = ffma2(pk2(__uint_as_float(a[2 * j]), __uint_as_float(a[2 * j + 1])), pk2(f, f), mm2);
               }
-              if (c + 32 < BK) tmem_ld32(S + c + 32, a);  // under this chunk's exponentials
+              if (c + 32 < SB) tmem_ld32(S + c + 32, a);  // under this chunk's exponentials
               uint32_t o[16];
 #pragma unroll
               for (int j = 0; j < 16; j++) {
@@ -513,13 +520,16 @@ __global__ void __launch_bounds__(THREADS, 1)
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(pfull + half);
+          if (lane == 0) mbar_arrive(pfull + 2 * half + buf);
         }
-        if (ok && !wait_phase(ofull + half, pieces & 1, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN)) ok = false;
+        ring += nb;
+        // the last two products one after the other: a phase can only be waited for while the one before it is over
+        for (uint32_t n = it - 2; n != it; n++)
+          if (ok && !wait_phase(odone + half, n & 1, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN)) ok = false;
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
-        pieces++, ring_piece++;
+        ring_piece++;
       }
       // ---- the row's result, whole or for the join
       const bool whole = w.off == 0 && take == t.cost;
