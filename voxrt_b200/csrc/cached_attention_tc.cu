@@ -1,16 +1,21 @@
 // Attention over the paged int8 cache for many queries: tiles of 256 (query, query head) rows on tcgen05.
 //
-// A CTA holds two halves of 128 rows. Per block of 128 keys, one warp brings the codes by TMA, four turn them into f16
+// A CTA holds two halves of 128 rows. Per block of 128 keys, one warp brings the codes by TMA and four turn them into f16
 // operands in shared memory (keys as they are, values times v_scale / ref * 2^8 with ref the largest value scale of the
-// piece, rounding 2^-11), one thread issues S = Q K^T and O += P V for both halves in turn, and a warpgroup a half does the softmax: a thread
-// owns a row, reads its 128 scores from TMEM twice (maximum, then exponentials) and writes the probabilities back over
-// them as f16, which is the second product's operand. While one half is in its softmax the tensor cores work for the
-// other. The row's reference maximum only moves when a score exceeds it by more than 8 (in powers of two): probabilities
-// then are at most 2^8, times 2^7 for the sake of f16's small end, and O is rarely rescaled. Softmax sums, scores and O are
-// f32. Query rows are scaled by a power of two like in the few-row kernels.
+// piece, rounding 2^-11). One warp issues S = Q K^T and O += P V for both halves in turn, in steps of 64 keys, and a
+// warpgroup a half does the softmax: a thread owns a row, reads its 64 scores of a step from TMEM twice (maximum, then
+// exponentials) and writes the probabilities back over them as f16, which is the second product's operand. A half has two
+// score buffers, so that the next step's scores are ready when a softmax ends. The row's reference only moves when a score
+// exceeds it by more than 2^8: probabilities are at most that, times 2^7 for the sake of f16's small end, and O is rarely
+// rescaled. Softmax sums, scores and O are f32. Query rows are scaled by a power of two like in the other kernels.
 //
-// TMEM (512 columns): S and P of the halves at 0 and 128, O at 256 and 256 + HD. A half's next S overwrites its P: the
-// tensor cores run one thread's products in order, and the commit that reports S also reports the product before it.
+// TMEM (512 columns): scores of a half at 128 half and 64 columns on, O at 256 + HD half. A step's scores overwrite the
+// probabilities of the step before last: the tensor cores run one thread's products in order.
+//
+// Bound by the softmax warps, of which registers and TMEM allow two a scheduler: per 128 keys and 256 rows the tensor
+// cores need 2048 clocks (measured alone) and the exponentials as many (16 a clock), the kernel takes about 5600. Longer
+// unrolled loops were slower each time (instruction fetches of four roles), as were sixteen softmax warps of half rows,
+// one pass over scores held in registers, and part of the exponentials by polynomial.
 #include <cuda_runtime.h>
 
 #include "cached_attention.cuh"
@@ -39,7 +44,7 @@ struct Layout {
   static constexpr uint32_t VF = KS + RING * 32;          // [RING][8] f32: their value scales / ref * 2^8
   static constexpr uint32_t REF = VF + RING * 32;         // [RING] f32
   static constexpr uint32_t BARS = REF + RING * 4;
-  static constexpr uint32_t BYTES = BARS + 25 * 8 + 1024;
+  static constexpr uint32_t BYTES = BARS + 27 * 8 + 1024;
   static_assert(BYTES <= 232448, "shared memory budget");
 };
 
@@ -84,6 +89,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint64_t *qfull = bars + 8, *sfull = bars + 10, *pfull = bars + 14, *odone = bars + 18;  // by half; sfull, pfull: and buffer
   uint64_t* drain = bars + 20;
   uint64_t *rkfull = bars + 21, *rkempty = bars + 22, *rvfull = bars + 23, *rvempty = bars + 24;
+  uint64_t* ofull = bars + 25;  // by half: the last product of a piece
   __shared__ Piece first_s;
   __shared__ uint32_t holder;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -97,6 +103,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(vempty + i, 1);
       mbar_init(qfull + i, 4);
       mbar_init(odone + i, 1);
+      mbar_init(ofull + i, 1);
     }
     for (int i = 0; i < 4; i++) {
       mbar_init(sfull + i, 1);
@@ -290,13 +297,14 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       __syncwarp();
     };
-    auto values = [&](int half, uint32_t n, int st, int sub, bool fresh) {
+    auto values = [&](int half, uint32_t n, int st, int sub, bool fresh, bool last) {
       const uint64_t v = desc_mn + (Lay::V + st * Lay::OPER + sub * SB * 128) / 16;
       if (leader) {
 #pragma unroll
         for (int j = 0; j < SB / 16; j++)
           mma_f16_ts(tmem + 256 + half * HD, tmem + half * 128 + (n & 1) * SB + 8 * j, v + j * 128, PV, fresh && j == 0 ? 0u : 1u);
         mma_commit(odone + half);
+        if (last) mma_commit(ofull + half);
       }
       __syncwarp();
     };
@@ -321,7 +329,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const bool more = i + 2 < ns;
         if (sub == 0 && !wait(vfull + st, it >> 1)) break;
         if (!wait(pfull + (n0 & 1), n0 >> 1)) break;
-        values(0, n0, st, sub, i == 0);
+        values(0, n0, st, sub, i == 0, i + 1 == ns);
         if (more) {  // the step after next, over the probabilities that these products read
           if (sub == 0 && !wait(kfull + (st ^ 1), (it + 1) >> 1)) break;
           scores(0, n0 + 2, st ^ 1, sub);
@@ -329,7 +337,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         n0++;
         if (two) {
           if (!wait(pfull + 2 + (n1 & 1), n1 >> 1)) break;
-          values(1, n1, st, sub, i == 0);
+          values(1, n1, st, sub, i == 0, i + 1 == ns);
           if (more) scores(1, n1 + 2, st ^ 1, sub);
           n1++;
         }
@@ -351,7 +359,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t lanes = (uint32_t)wrow << 16;
     const uint32_t S0 = tmem + lanes + half * 128, O = tmem + lanes + 256 + half * HD;
     bool ok = true;
-    uint32_t it = 0;                     // steps of this half so far
+    uint32_t it = 0, pieces = 0;         // steps and pieces of this half so far
     uint32_t ring = 0, ring_piece = 0;   // blocks and pieces with keys of the CTA so far
     for (Piece w = first; w.left > 0 && ok; w.next(p, MT, BK)) {
       const Tile& t = w.t;
@@ -523,13 +531,12 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (lane == 0) mbar_arrive(pfull + 2 * half + buf);
         }
         ring += nb;
-        // the last two products one after the other: a phase can only be waited for while the one before it is over
-        for (uint32_t n = it - 2; n != it; n++)
-          if (ok && !wait_phase(odone + half, n & 1, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN)) ok = false;
+        // a barrier of its own: when a warp comes here, odone may be one or two phases behind
+        if (ok && !wait_phase(ofull + half, pieces & 1, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN)) ok = false;
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
-        ring_piece++;
+        ring_piece++, pieces++;
       }
       // ---- the row's result, whole or for the join
       const bool whole = w.off == 0 && take == t.cost;
