@@ -33,7 +33,8 @@ def _case(seed, m, n, k, lo=-127):
 SHAPES = [(1, 1, 16), (1, 17, 48), (2, 40, 16), (7, 33, 1040), (8, 128, 128), (9, 100, 144), (16, 1000, 4096),
           (17, 24, 272), (31, 640, 2048), (33, 129, 96), (64, 256, 1024), (65, 130, 176), (127, 257, 400),
           (128, 256, 256), (129, 255, 4112), (200, 1024, 640), (256, 512, 128), (257, 300, 2064), (600, 700, 336),
-          (1000, 1031, 1024), (4, 2048, 16384), (300, 264, 16384)]
+          (1000, 1031, 1024), (4, 2048, 16384), (300, 264, 16384), (100, 50, 16), (300, 17, 32),
+          (20, 2080, 48), (44, 4100, 1040), (513, 2049, 272)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
