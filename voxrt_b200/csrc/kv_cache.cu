@@ -10,7 +10,8 @@
 //
 // Bound by memory for long runs, by the chain of dependent loads (offsets, page table, values) for single tokens: one
 // block takes one page of K or V and a run of heads, finds its sequence with 32 probes a step, and holds a head's new values
-// in registers between the maximum and the codes, with the next head's on their way.
+// in registers between the maximum and the codes, with the next head's on their way. Measured: 64 sequences of one token
+// 5.3 us; 8 ragged sequences of up to 2048 tokens, 8 heads of 128, 24.6 us (100 MB, 4 TB/s), read back 20.8 us (5.2 TB/s).
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -307,7 +308,8 @@ vxg_status vxg_cache_write(const vxg_kv_cache* c, const void* k, long long ld_k,
     constexpr int DT = decltype(tag)::value;
     cudaStream_t st = (cudaStream_t)stream;
     const int most = std::min(total, c->page) * c->head_dim / 8;  // vectors of a page and head
-    // a few tokens a sequence: small blocks, which all fit the GPU at once; measured, 64 sequences of one token: see above
+    // a few tokens a sequence: small blocks, which all fit the GPU at once (64 sequences of one token: 5.3 us, 10.3 us with
+    // blocks of 256)
     if (total <= 4LL * n_seq) cache::write_launch<DT, 64, 1, true>(p, (int)items, vec, st);
     else if (most <= 512) cache::write_launch<DT, 256, 2, false>(p, (int)items, vec, st);
     else if (most <= 1024) cache::write_launch<DT, 256, 4, false>(p, (int)items, vec, st);
