@@ -8,7 +8,7 @@
 // (f32 queries, which need more than 16 bits of it, subtract). P^T comes out of S^T by an 8 x 8 transpose within the warp.
 // The warps' states meet in shared memory at the end of a piece. Measured: 64 ragged sequences over up to 16000 tokens, 8
 // cache heads of 128 for 32 query heads, 241 us (1.28 GB, 5.3 TB/s); f32 queries 318 us; one sequence over 1500 tokens, 16
-// heads of 64, 12 us, which is the chain of dependent loads of the two kernels.
+// heads of 64, 12 us, the chain of dependent loads of the two kernels for the most part.
 #include <cuda_runtime.h>
 
 #include "cached_attention.cuh"

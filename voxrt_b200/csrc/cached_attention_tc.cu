@@ -13,8 +13,9 @@
 // probabilities of the step before last: the tensor cores run one thread's products in order.
 //
 // Bound by the softmax warps, of which registers and TMEM allow two a scheduler: per 128 keys and 256 rows the tensor
-// cores need 2048 clocks (measured alone) and the exponentials as many (16 a clock); the kernel takes about 5600 (4 x 2048 queries of 32 heads over 1000 .. 4000 tokens: 389 us, 470 TFLOP/s of what is
-// visible). Longer
+// cores need 2048 clocks (measured alone) and the exponentials as many (16 a clock); the kernel takes about 5800 with its
+// pieces' ends (4 ragged sequences of up to 2048 queries of 32 heads behind up to 2000 cached tokens: 389 us, 520 TFLOP/s of
+// what is visible). Longer
 // unrolled loops were slower each time (instruction fetches of four roles), as were sixteen softmax warps of half rows,
 // one pass over scores held in registers, and part of the exponentials by polynomial.
 #include <cuda_runtime.h>

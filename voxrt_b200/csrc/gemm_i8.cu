@@ -7,7 +7,7 @@
 // warps share the K axis, and the weights go from memory straight into the operand registers of mma.m16n8k32: the words of a
 // thread's 16-byte load of a channel are its k slots of two steps, and as the token operand is loaded in the same order the
 // permutation of k cancels. The warps' partial sums meet in shared memory. Measured: one token, 16384 x 8192 weights
-// (not in L2) 23.5 us, 5.7 TB/s; 4096 x 4096 (in L2) 4.8 us; 37 tokens, 8192 x 2048, 7.1 us.
+// (larger than L2) 23.7 us, 5.7 TB/s; 4096 x 4096 (in L2) 4.9 us; 37 tokens, 8192 x 2048, 7.1 us.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -140,9 +140,10 @@ vxg_status launch_few(const Params& p, cudaStream_t st) {
 // int32 sums. Sharing w this way halves the operand bytes an SM reads per product, which is what limits a single CTA's
 // 128 x 256 tile. Persistent over tiles, two TMEM buffers, so a tile's epilogue runs under the next one's products.
 // Roles: warps 0-7 epilogue (TMEM lanes 32 (w % 4).., column half w / 4), warp 8 TMA producer, warp 9 MMA issuer (leader).
-// Measured, 8192 x 16384 x 4096: 346 us, 3.2 POP/s, 93 % of twice what the bf16 library product reaches (tensor pipe 88 %
-// busy in isolation); 1500 x 1024 x 4096: 11.1 us, where a tile's 16 stages take their fill time, not the products'. A wait
-// and a commit for every 128 k instead of 256 cost a third more at small tiles: issuing was the bound.
+// Measured, 8192 x 16384 x 4096: 346 .. 356 us, 3.1 .. 3.2 POP/s, 90 .. 93 % of twice the bf16 library product's rate (8192 x
+// 8192 x 4096 alone: tensor pipe 88 % busy); 1500 x 1024 x 4096: 11.1 us, of which a tile's 16 stages are 6 and the rest is
+// launch, fill and epilogue. Stages of 128 k, with a wait and a commit each, were slower at small tiles, where issuing is the
+// bound (256 x 512 x 16384: 32.8 against 23.5 us).
 namespace tc {
 
 constexpr int BM = 256, BK = 256, SUB = 128, EPI_WARPS = 8, THREADS = (EPI_WARPS + 2) * 32;

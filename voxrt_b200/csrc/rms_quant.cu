@@ -11,8 +11,8 @@
 // Bound by memory: x and v are read once, the sum, the codes and the normalised row written once, and a row stays in
 // registers (eight elements a thread and vector) between the two reductions. A row of up to 256 elements belongs to
 // one warp, a longer one to a block. Measured: 16384 x 4096 bf16 with residual 102 us (470 MB, 4.6 TB/s), 8192 x 4096 f32
-// 87 us (5.0 TB/s), one row of 1024 2.9 us; what holds the 16-bit rows below the copy rate is issue (68 % of the slots busy).
-// The 64-bit sum costs 3 %.
+// 87 us (5.0 TB/s), one row of 1024 2.9 us. 16-bit rows are held below the copy rate by issue (68 % of the slots busy):
+// with the squares summed in f32 the first would take 97 us, the second is the same.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -324,7 +324,8 @@ static vxg_status run(Params p, int dtype, bool norm, cudaStream_t st) {
   const int vecs = (p.d + 7) / 8, lanes = p.group / 8;
   p.lanes = p.group < p.d && lanes <= 32 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
   // Many rows: 256 threads a row, whose barriers are cheaper; few (fewer than four an SM): 512, which shortens a row's
-  // own time. Measured, 4096 columns, bf16: 16384 rows 114 against 132 us, one row 4.0 against 3.7 us.
+  // own time. Measured, 4096 columns, bf16: 16384 rows 114 against 132 us, one row 4.0 against 3.7 us
+  // (both sides before the codes' fast rounding, which brought the first to 102).
   const int most = p.n < 4 * sm_count() ? 512 : 256;
   int nv = 1;
   while (nv < 8 && (vecs + nv - 1) / nv > most) nv *= 2;
