@@ -251,6 +251,32 @@ def test_extreme_queries(KvCache, dtype):
         assert (np.abs(got - want) <= bound).all(), h
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("length", ["one block", 300])  # whole tiles, tiles of several shares
+@pytest.mark.parametrize("hd,heads,new", [(64, 2, 3), (128, 2, 7), (64, 2, 20), (128, 2, 20), (64, 2, 80), (128, 2, 80)])
+def test_smallest_value_scales(KvCache, hd, heads, new, length, dtype):
+    """Value scales from the smallest that a write leaves, 2^-126, on, in tiles of every size. Everything is compared times
+    2^118, the oracle with scales that are larger by as much (exact). On top of its bound: results below 2^-126 are
+    subnormal, off by half a step of 2^-149 (bf16: 2^-133), and so are up to 64 joined parts in f32."""
+    length = (60 if new < 60 else 100) if length == "one block" else length
+    rng = np.random.default_rng(hd + new)
+    table, n_pages = _table(rng, [length], 32)
+    ref, c = _pair(KvCache, rng, n_pages, 1, 32, hd)
+    ref.scales[0] *= np.float32(0.02)
+    ref.scales[1] = (2.0 ** -126 * rng.uniform(1, 4, ref.scales[1].shape)).astype(np.float32)
+    ref.scales[1][table[0, 0]] = np.float32(2.0 ** -126)
+    c.ks.copy_(torch.from_numpy(ref.scales[0]))
+    c.vs.copy_(torch.from_numpy(ref.scales[1]))
+    q = torch.from_numpy(rng.standard_normal((new, heads, hd)).astype(np.float32)).to(dtype).cuda()
+    cu = [0, new]
+    got = f32(c.attend(q, _int(table), _int([length]), _int(cu), scale=0.11)).astype(np.float64) * 2.0 ** 118
+    ref.scales[1] = ref.scales[1] * np.float32(2.0 ** 118)
+    want, bound = attend(ref, f32(q), table, [length], cu, float(np.float32(0.11)), True, 0, dtype)
+    bound += 2.0 ** 118 * (64 * 2.0 ** -150 + (2.0 ** -134 if dtype == torch.bfloat16 else 2.0 ** -150))
+    _ok()
+    assert (np.abs(got - want) <= bound).all()
+
+
 def test_shared_pages_other_stream_and_graph(KvCache):
     """Two sequences over the same prefix pages; a captured call replayed with other lengths; a side stream."""
     rng = np.random.default_rng(10)

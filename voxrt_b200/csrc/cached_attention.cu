@@ -217,9 +217,10 @@ __global__ void __launch_bounds__(THREADS, 2)
       if (__any_sync(0xffffffffu, wider || mx[0] > S.m[0] + 8.0f || mx[1] > S.m[1] + 8.0f)) {
         float reff = 1.0f;
         if (wider) {  // the same in the whole warp
-          reff = S.ref / vsm;
-          inv_ref = 128.0f / vsm;  // finite: a page's scale is 0 or at least 2^-126
-          S.ref = vsm;
+          const float old = S.ref;
+          S.ref = fmaxf(vsm, 1.17549435e-38f);  // what a written page has at least, so that the reciprocal is finite
+          inv_ref = 1.0f / S.ref;
+          reff = old / S.ref;
         }
 #pragma unroll
         for (int e = 0; e < 2; e++) {
@@ -236,7 +237,7 @@ __global__ void __launch_bounds__(THREADS, 2)
       // ---- probabilities, times 2^7 and the value scale, and the second product, 16 keys a step
 #pragma unroll
       for (int kk = 0; kk < TOK / 16; kk++) {
-        const float vf = scales[4 + kk] * inv_ref;
+        const float vf = scales[4 + kk] * inv_ref * 128.0f;
         uint32_t pa[4], pb[4];
 #pragma unroll
         for (int e = 0; e < 2; e++)  // key group 2 kk + e
@@ -294,7 +295,7 @@ __global__ void __launch_bounds__(THREADS, 2)
       S.l[e] += __shfl_xor_sync(0xffffffffu, S.l[e], 1);
       S.l[e] += __shfl_xor_sync(0xffffffffu, S.l[e], 2);
     }
-    const float unit = S.ref * (1.0f / 128.0f);
+    const float unit = 1.0f / 128.0f;  // and S.ref last: their product may be too small for f32's digits
     const bool whole = off == 0 && take == t.cost;
     float* part = p.part + ((size_t)blockIdx.x * MAX_PIECES + (w.first ? 0 : 1)) * MT * (HD + 2);
     // thread (g, c)'s columns: HD / 4 consecutive ones, the first HD / 8 in o[.][0 or 2], the rest in o[.][1 or 3]
@@ -311,7 +312,7 @@ __global__ void __launch_bounds__(THREADS, 2)
               for (int j = 0; j < HD / 8; j += 8) {
                 float a[8], b2[8];
     #pragma unroll
-                for (int k = 0; k < 8; k++) a[k] = S.o[j + k][2 * e] * inv, b2[k] = S.o[j + k][2 * e + 1] * inv;
+                for (int k = 0; k < 8; k++) a[k] = S.o[j + k][2 * e] * inv * S.ref, b2[k] = S.o[j + k][2 * e + 1] * inv * S.ref;
                 store8<DT>(o + j, a);
                 store8<DT>(o + HD / 8 + j, b2);
               }
@@ -321,8 +322,8 @@ __global__ void __launch_bounds__(THREADS, 2)
               o += 2 + c * (HD / 4);
     #pragma unroll
               for (int j = 0; j < HD / 8; j++) {
-                o[j] = S.o[j][2 * e] * unit;
-                o[HD / 8 + j] = S.o[j][2 * e + 1] * unit;
+                o[j] = S.o[j][2 * e] * unit * S.ref;
+                o[HD / 8 + j] = S.o[j][2 * e + 1] * unit * S.ref;
               }
             }
           }

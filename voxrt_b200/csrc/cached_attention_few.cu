@@ -232,9 +232,10 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? FEW_CTAS_8 : 2)
       if (__any_sync(0xffffffffu, over || wider)) {
         float reff = 1.0f;
         if (wider) {  // the same in the whole warp
-          reff = ref / vs;
-          inv_ref = 128.0f / vs;  // finite: a page's scale is 0 or at least 2^-126
-          ref = vs;
+          const float old = ref;
+          ref = fmaxf(vs, 1.17549435e-38f);  // what a written page has at least, so that the reciprocal is finite
+          inv_ref = 1.0f / ref;
+          reff = old / ref;
         }
 #pragma unroll
         for (int n = 0; n < NQ; n++)
@@ -253,7 +254,7 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? FEW_CTAS_8 : 2)
           }
       }
       // ---- probabilities, times 2^7 and the value scale for the second product
-      const float vf = vs * inv_ref;
+      const float vf = vs * inv_ref * 128.0f;
       uint32_t pb[NQ][2], pr[SPLIT ? NQ : 1][2];
 #pragma unroll
       for (int n = 0; n < NQ; n++) {
@@ -296,7 +297,7 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? FEW_CTAS_8 : 2)
     }
     if (!ok && lane == 0) fail = 1;  // read behind the second barrier below: all give up together
     // ---- the warps' states meet
-    const float unit = ref * (1.0f / 128.0f);
+    auto result = [&](float x) { return x * (1.0f / 128.0f) * ref; };  // ref / 128 alone may be too small for f32's digits
     const bool whole = off == 0 && take == t.cost;
     float* part = p.part + ((size_t)blockIdx.x * MAX_PIECES + (w.first ? 0 : 1)) * MT * (HD + 2);
     float* mo = reinterpret_cast<float*>(smem + Lay::MERGE);
@@ -311,8 +312,7 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? FEW_CTAS_8 : 2)
         float* row = mo + r * LD + (HD / 8) * g;
 #pragma unroll
         for (int i = 0; i < KS; i += 2)
-          *reinterpret_cast<float4*>(row + 2 * i) = make_float4(o[n][i][e] * unit, o[n][i][2 + e] * unit,
-                                                                o[n][i + 1][e] * unit, o[n][i + 1][2 + e] * unit);
+          *reinterpret_cast<float4*>(row + 2 * i) = make_float4(result(o[n][i][e]), result(o[n][i][2 + e]), result(o[n][i + 1][e]), result(o[n][i + 1][2 + e]));
         if (g == 0) ms[2 * r] = m[n][e], ms[2 * r + 1] = l[n][e];
       }
     named_bar_sync(1, CONS * 32);

@@ -375,7 +375,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const long long pos = (long long)t.L - t.n + i;
       const int khi = p.causal ? (int)::max(0LL, ::min((long long)t.L, pos + 1)) : t.L;
       const int klo = p.window > 0 ? (int)::max(0LL, pos - p.window + 1) : 0;
-      float m = -INFINITY, l = 0.0f, unit = 0.0f;
+      float m = -INFINITY, l = 0.0f, ref = 0.0f;
       if (nb > 0) {
         // ---- the warp's rows of Q: each scaled by a power of two, f16, into the half's operand. LPR lanes read a row.
         const long long qoff = live ? (long long)(t.q0 + i) * p.ld_q + (long long)head * HD : -1;
@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           const int key0 = (t.blk0 + w.off) * BK + b * SB;
           const bool inside = key0 >= all_lo && key0 + SB <= all_hi;
           const float* ks = ks_s + ((ring + b / 2) % RING) * 8 + (b & 1) * (SB / 16);
-          if (b == 0) unit = ref_s[ring_piece % RING] * (1.0f / 256.0f);
+          if (b == 0) ref = ref_s[ring_piece % RING];
           // ---- the step's maximum
           float mx = -INFINITY;
           auto maximum = [&](auto tag) {
@@ -543,7 +543,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       // ---- the row's result, whole or for the join
       const bool whole = w.off == 0 && take == t.cost;
       float* part = p.part + ((size_t)blockIdx.x * MAX_PIECES + (w.first ? 0 : 1)) * MT * (HD + 2) + (size_t)r * (HD + 2);
-      const float inv = l == 0.0f ? 0.0f : unit / l;
+      const float inv = l == 0.0f ? 0.0f : (1.0f / 256.0f) / l;  // ref last: their product may be too small for f32's digits
       if (live && !whole) part[0] = m - 7.0f, part[1] = l;
       uint8_t* os = smem + Lay::Q + half * Lay::OPER;  // the half's products are done with Q
 #pragma unroll 1
@@ -562,7 +562,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             uint32_t h[4];
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-              const float v0 = __uint_as_float(a[j + 2 * k]) * inv, v1 = __uint_as_float(a[j + 2 * k + 1]) * inv;
+              const float v0 = __uint_as_float(a[j + 2 * k]) * inv * ref, v1 = __uint_as_float(a[j + 2 * k + 1]) * inv * ref;
               h[k] = narrow2<DT>(l == 0.0f ? 0.0f : v0, l == 0.0f ? 0.0f : v1);
             }
             *reinterpret_cast<uint4*>(os + (c / 64) * Lay::HALF +
@@ -573,7 +573,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
           for (int j = 0; j < 32; j += 2)
             *reinterpret_cast<float2*>(part + 2 + c + j) =
-                make_float2(__uint_as_float(a[j]) * unit, __uint_as_float(a[j + 1]) * unit);
+                make_float2(__uint_as_float(a[j]) * (1.0f / 256.0f) * ref, __uint_as_float(a[j + 1]) * (1.0f / 256.0f) * ref);
         }
         __syncwarp();
       }
