@@ -85,9 +85,8 @@ class Cache:
 def attend(cache, q, table, lens, cu, scale, causal, window, dtype):
     """(out, bound) in 64 bits; `bound` is how far the library's result may be off, element by element.
 
-    Per probability: f16 rounding, 11 significant bits and so at most 2^-11, and the same for a value times its scale where
-    the tiles are large, 2^-10 together (f32 queries: two parts, 2^-22), and the error of its score, twice (numerator and
-    denominator). A score is a sum of hd exact products in f32, in the tensor cores' order: at most (hd + 8) half-steps
+    Per probability: f16 rounding, 11 significant bits and so at most 2^-11 (f32 queries: two parts, 2^-22), and the error of
+    its score, twice (numerator and denominator). Codes are exact, and the value scales enter in f32 before that rounding. A score is a sum of hd exact products in f32, in the tensor cores' order: at most (hd + 8) half-steps
     of truncation (2^-23) of sum |q k|, and for 16-bit queries, whose codes enter as 1152 + code against a start of -1152
     times the row's sum, of 16 partial sums of size 1152 sum |q| k_scale more; exp2 and the scale products add less than 2^-20 relative for the scores' size met
     here. A probability is rounded in units of 2^-7 (at the coarsest) of the largest value scale `ref`: f16's finest step
@@ -97,7 +96,7 @@ def attend(cache, q, table, lens, cu, scale, causal, window, dtype):
     rows, heads, hd = q.shape
     share = heads // cache.heads
     out, bound = np.zeros((rows, heads, hd)), np.zeros((rows, heads, hd))
-    prob = 2.0 ** -22 if dtype == torch.float32 else 2.0 ** -10
+    prob = 2.0 ** -22 if dtype == torch.float32 else 2.0 ** -11
     for s in range(len(lens)):
         L, n = int(lens[s]), int(cu[s + 1] - cu[s])
         if n == 0 or L == 0:

@@ -1,13 +1,15 @@
 // Attention over the paged int8 cache for many queries: tiles of 256 (query, query head) rows on tcgen05.
 //
 // A CTA holds two halves of 128 rows. Per block of 128 keys, one warp brings the codes by TMA and four turn them into f16
-// operands in shared memory (keys as they are, values times v_scale / ref * 2^8 with ref the largest value scale of the
-// piece, rounding 2^-11). One warp issues S = Q K^T and O += P V for both halves in turn, in steps of 64 keys, and a
-// warpgroup a half does the softmax: a thread owns a row, reads its 64 scores of a step from TMEM twice (maximum, then
-// exponentials) and writes the probabilities back over them as f16, which is the second product's operand. A half has two
-// score buffers, so that the next step's scores are ready when a softmax ends. The row's reference only moves when a score
-// exceeds it by more than 2^8: probabilities are at most that, times 2^7 for the sake of f16's small end, and O is rarely
-// rescaled. Softmax sums, scores and O are f32. Query rows are scaled by a power of two like in the other kernels.
+// operands in shared memory, which is exact. One warp issues S = Q K^T and O += P V for both halves in turn, in steps of 64
+// keys, and a warpgroup a half does the softmax: a thread owns a row, reads its 64 scores of a step from TMEM twice
+// (maximum, then exponentials) and writes the probabilities back over them as f16, the second product's operand, times
+// v_scale / ref with ref the largest value scale of the piece. That is the one rounding of an operand (2^-11): with the
+// values scaled before the product there were two more, and f16 results were off by 3.2e-4 of their norm instead of 2.7e-4,
+// at the same speed. A half has two score buffers, so that the next step's scores are ready when a softmax ends. The row's
+// reference only moves when a score exceeds it by more than 2^8: probabilities are at most that, times 2^7 for the sake of
+// f16's small end, and O is rarely rescaled. Softmax sums, scores and O are f32. Query rows are scaled by a power of two
+// like in the other kernels.
 //
 // TMEM (512 columns): scores of a half at 128 half and 64 columns on, O at 256 + HD half. A step's scores overwrite the
 // probabilities of the step before last: the tensor cores run one thread's products in order.
@@ -15,9 +17,8 @@
 // Bound by the softmax warps, of which registers and TMEM allow two a scheduler: per 128 keys and 256 rows the tensor
 // cores need 2048 clocks (measured alone) and the exponentials as many (16 a clock); the kernel takes about 5800 with its
 // pieces' ends (4 ragged sequences of up to 2048 queries of 32 heads behind up to 2000 cached tokens: 389 us, 520 TFLOP/s of
-// what is visible). Longer
-// unrolled loops were slower each time (instruction fetches of four roles), as were sixteen softmax warps of half rows,
-// one pass over scores held in registers, and part of the exponentials by polynomial.
+// what is visible). Slower: longer unrolled loops (instruction fetches of four roles), one pass over scores held in
+// registers. No gain: sixteen softmax warps of half rows, a quarter of the exponentials by polynomial.
 #include <cuda_runtime.h>
 
 #include "cached_attention.cuh"
@@ -43,7 +44,7 @@ struct Layout {
   static constexpr uint32_t RAW = 128 * HD;               // a block's codes
   static constexpr uint32_t RK = V + 2 * OPER, RV = RK + RAW;
   static constexpr uint32_t KS = RV + RAW;                // [RING][8] f32: key scales of the block's 16-key pieces
-  static constexpr uint32_t VF = KS + RING * 32;          // [RING][8] f32: their value scales / ref * 2^8
+  static constexpr uint32_t VF = KS + RING * 32;          // [RING][8] f32: their value scales / ref
   static constexpr uint32_t REF = VF + RING * 32;         // [RING] f32
   static constexpr uint32_t BARS = REF + RING * 4;
   static constexpr uint32_t BYTES = BARS + 27 * 8 + 1024;
@@ -176,7 +177,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (!ok) break;
       if (lane < CHUNKS) {
         ks_s[(it % RING) * 8 + lane] = ks;
-        vf_s[(it % RING) * 8 + lane] = ref > 0.0f ? vs / ref * 256.0f : 0.0f;
+        vf_s[(it % RING) * 8 + lane] = ref > 0.0f ? vs / ref : 0.0f;
       }
       if (lane == 8 && x.b == 0) ref_s[x.piece % RING] = ref;
       __syncwarp();
@@ -209,20 +210,13 @@ __global__ void __launch_bounds__(THREADS, 1)
     };
     // 16 codes -> two 16-byte chunks of the operand row; the upper half of the lanes of a key stores its odd chunk first,
     // so that the eight lanes of a store phase meet eight different chunks
-    auto put = [&](uint8_t* dst, int k, uint4 x, bool scaled, __half2 f) {
+    auto put = [&](uint8_t* dst, int k, uint4 x) {
       const uint32_t w[4] = {swap ? x.z : x.x, swap ? x.w : x.y, swap ? x.x : x.z, swap ? x.y : x.w};
       uint32_t h[8];
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         h[2 * i] = codes_to_f16(__byte_perm(w[i], 0, 0x4140));
         h[2 * i + 1] = codes_to_f16(__byte_perm(w[i], 0, 0x4342));
-      }
-      if (scaled) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const __half2 v = __hmul2(*reinterpret_cast<__half2*>(&h[i]), f);
-          h[i] = *reinterpret_cast<const uint32_t*>(&v);
-        }
       }
       uint8_t* base = dst + (e0 / 64) * Lay::HALF;
       const uint32_t c = (uint32_t)(e0 % 64) / 8;
@@ -244,7 +238,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll 2  // more would cost more in instruction fetches than it hides
       for (int i = 0; i < PASSES; i++) {
         const int k = i * CONV_WARPS * KPW + kk;
-        put(dk, k, get(smem + Lay::RK, k), false, __half2());
+        put(dk, k, get(smem + Lay::RK, k));
       }
       fence_proxy_async_smem();
       __syncwarp();
@@ -255,11 +249,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (it >= 2 && !wait(vempty + st, (it >> 1) - 1)) break;
       if (!wait(rvfull, it)) break;
       uint8_t* dv = smem + Lay::V + st * Lay::OPER;
-      const float* vf = vf_s + (it % RING) * 8;
 #pragma unroll 2
       for (int i = 0; i < PASSES; i++) {
         const int k = i * CONV_WARPS * KPW + kk;
-        put(dv, k, get(smem + Lay::RV, k), true, __float2half2_rn(vf[k / 16]));
+        put(dv, k, get(smem + Lay::RV, k));
       }
       fence_proxy_async_smem();
       __syncwarp();
@@ -433,7 +426,8 @@ __global__ void __launch_bounds__(THREADS, 1)
           tc_fence_after();
           const int key0 = (t.blk0 + w.off) * BK + b * SB;
           const bool inside = key0 >= all_lo && key0 + SB <= all_hi;
-          const float* ks = ks_s + ((ring + b / 2) % RING) * 8 + (b & 1) * (SB / 16);
+          const int scales = ((ring + b / 2) % RING) * 8 + (b & 1) * (SB / 16);
+          const float *ks = ks_s + scales, *vf = vf_s + scales;
           if (b == 0) ref = ref_s[ring_piece % RING];
           // ---- the step's maximum
           float mx = -INFINITY;
@@ -497,7 +491,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll 1
             for (int c = 0; c < SB; c += 32) {
               uint64_t x[16];
-              const float f0 = rowf * ks[c / 16], f1 = rowf * ks[c / 16 + 1];
+              const float f0 = rowf * ks[c / 16], f1 = rowf * ks[c / 16 + 1], g0 = vf[c / 16], g1 = vf[c / 16 + 1];
               tmem_wait_ld();
 #pragma unroll
               for (int j = 0; j < 16; j++) {
@@ -517,7 +511,9 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
                 const float p0 = ex2(x0), p1 = ex2(x1);
                 sum[j & 3] = fadd2(sum[j & 3], pk2(p0, p1));
-                o[j] = pack_f16(p0, p1);
+                float y0, y1;
+                upk2(fmul2(pk2(p0, p1), j < 8 ? pk2(g0, g0) : pk2(g1, g1)), y0, y1);
+                o[j] = pack_f16(y0, y1);
               }
               tmem_st16(S + c / 2, o);
             }
@@ -543,7 +539,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       // ---- the row's result, whole or for the join
       const bool whole = w.off == 0 && take == t.cost;
       float* part = p.part + ((size_t)blockIdx.x * MAX_PIECES + (w.first ? 0 : 1)) * MT * (HD + 2) + (size_t)r * (HD + 2);
-      const float inv = l == 0.0f ? 0.0f : (1.0f / 256.0f) / l;  // ref last: their product may be too small for f32's digits
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // ref last: their product may be too small for f32's digits
       if (live && !whole) part[0] = m - 7.0f, part[1] = l;
       uint8_t* os = smem + Lay::Q + half * Lay::OPER;  // the half's products are done with Q
 #pragma unroll 1
@@ -573,7 +569,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
           for (int j = 0; j < 32; j += 2)
             *reinterpret_cast<float2*>(part + 2 + c + j) =
-                make_float2(__uint_as_float(a[j]) * (1.0f / 256.0f) * ref, __uint_as_float(a[j + 1]) * (1.0f / 256.0f) * ref);
+                make_float2(__uint_as_float(a[j]) * ref, __uint_as_float(a[j + 1]) * ref);
         }
         __syncwarp();
       }
