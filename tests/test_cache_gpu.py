@@ -277,6 +277,28 @@ def test_smallest_value_scales(KvCache, hd, heads, new, length, dtype):
     assert (np.abs(got - want) <= bound).all()
 
 
+@pytest.mark.parametrize("scale", [-0.3, 0.0])
+@pytest.mark.parametrize("hd,heads,new,dtype", [
+    (64, 2, 3, torch.float32), (128, 4, 2, torch.bfloat16), (128, 2, 7, torch.float16), (64, 2, 20, torch.bfloat16),
+    (64, 2, 80, torch.float32), (128, 2, 80, torch.float32), (128, 2, 20, torch.float16), (64, 4, 80, torch.float16),
+    (128, 4, 80, torch.bfloat16)])
+def test_scales_that_are_not_positive(KvCache, hd, heads, new, dtype, scale):
+    """Peaked scores under a negative scale, whose softmax follows the smallest products, and scale 0, which weighs every
+    key alike, in tiles of every size."""
+    rng = np.random.default_rng(hd + new + heads)
+    lens, count = [300, 150], [new, max(1, new - 3)]
+    table, n_pages = _table(rng, lens, 32)
+    ref, c = _pair(KvCache, rng, n_pages, 1, 32, hd)
+    ref.scales[0] *= np.float32(0.02)
+    c.ks.copy_(torch.from_numpy(ref.scales[0]))
+    cu = np.concatenate([[0], np.cumsum(count)])
+    q = torch.from_numpy(rng.standard_normal((int(cu[-1]), heads, hd)).astype(np.float32) * 1.5).to(dtype).cuda()
+    got = f32(c.attend(q, _int(table), _int(lens), _int(cu), scale=scale)).astype(np.float64)
+    want, bound = attend(ref, f32(q), table, lens, cu, float(np.float32(scale)), True, 0, dtype)
+    _ok()
+    assert (np.abs(got - want) <= bound).all()
+
+
 def test_shared_pages_other_stream_and_graph(KvCache):
     """Two sequences over the same prefix pages; a captured call replayed with other lengths; a side stream."""
     rng = np.random.default_rng(10)

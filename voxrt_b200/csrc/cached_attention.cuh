@@ -27,6 +27,7 @@ struct Params {
   int* status;
   int n_seq, max_pages, total, heads, share, window, causal, slots, grid;
   int page_log2;
+  int negate;  // tcgen05: scale_log2 is positive and the queries are negated
   float scale_log2;
 };
 
@@ -39,7 +40,7 @@ constexpr int FEW_CTAS_8 = 3;  // CTAs an SM, tiles of up to 8 rows
 // Tiles of up to 16 rows (cached_attention_few.cu).
 vxg_status launch_few(const Params& p, const Plan& pl, int head_dim, int dtype, cudaStream_t st);
 // 256-row tiles on tcgen05, f16 and bf16 queries (cached_attention_tc.cu).
-vxg_status launch_tc(const Params& p, const Plan& pl, int head_dim, int dtype, cudaStream_t st);
+vxg_status launch_tc(Params p, const Plan& pl, int head_dim, int dtype, cudaStream_t st);
 
 // Rows of codes [n_pages * heads * page][head_dim], copied in boxes of a page or `most` rows.
 inline vxg_status cache_map(CUtensorMap* map, const vxg_kv_cache& c, const int8_t* base, int most) {

@@ -21,6 +21,8 @@
 // registers. No gain: sixteen softmax warps of half rows, a quarter of the exponentials by polynomial.
 #include <cuda_runtime.h>
 
+#include <cmath>
+
 #include "cached_attention.cuh"
 
 namespace vxg {
@@ -265,7 +267,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     // --------------------------------------------------------------------------------------------- MMA issuer
     // The whole warp walks and waits, so that the operand descriptors stay in uniform registers, and one lane issues.
     // With one lane doing all of it, the descriptors' arithmetic took longer than the products.
-    constexpr uint32_t QK = idesc_f16(128, SB, false), PV = idesc_f16(128, HD, true);
+    // A negative `scale` negates Q here, so that the softmax's factors are positive: a step's maximum is taken of unscaled
+    // scores. Free here; negating Q where it is loaded was slower (4 x 2048 causal, 16 heads of 64: 208 us against 198).
+    constexpr uint32_t PV = idesc_f16(128, HD, true);
+    const uint32_t QK = idesc_f16(128, SB, false) | (p.negate ? 1u << 13 : 0u);  // negate A
     const bool leader = elect_one();
     // descriptor = fixed upper word, lower word = address / 16 and the offset between 64-column halves
     const uint64_t desc_k = umma_desc_sw128(smem_u32(smem)), desc_mn = umma_desc_sw128_mn(smem_u32(smem), Lay::HALF);
@@ -611,7 +616,9 @@ vxg_status launch(const Params& p, const Plan& pl, cudaStream_t st) {
 
 }  // namespace tc
 
-vxg_status launch_tc(const Params& p, const Plan& pl, int head_dim, int dtype, cudaStream_t st) {
+vxg_status launch_tc(Params p, const Plan& pl, int head_dim, int dtype, cudaStream_t st) {
+  p.negate = p.scale_log2 < 0.0f;
+  p.scale_log2 = std::fabs(p.scale_log2);
   if (head_dim == 128)
     return dtype == VXG_DT_BF16 ? tc::launch<128, VXG_DT_BF16>(p, pl, st) : tc::launch<128, VXG_DT_F16>(p, pl, st);
   return dtype == VXG_DT_BF16 ? tc::launch<64, VXG_DT_BF16>(p, pl, st) : tc::launch<64, VXG_DT_F16>(p, pl, st);
