@@ -144,6 +144,27 @@ def test_feeds_the_ternary_product(K, oracle_lib):
     assert bits_equal(f32(y), oracle_lib.gemm(w_rows, sw, q, s, 128))
 
 
+@pytest.mark.parametrize("d", [1, 8])  # element by element, and with the next row's look-ahead
+def test_most_rows(K, d):
+    """2^31 - 1 rows: the row index plus a step of the grid passes 31 bits. Only a few runs of the input are written, and
+    compared; the rest is whatever the memory holds."""
+    n = 2 ** 31 - 1
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < n * (3 * d + 4) * 1.2:
+        pytest.skip("not enough memory")
+    x = torch.empty((n, d), dtype=torch.float16, device="cuda")
+    runs = [slice(0, 1000), slice(2 ** 30 - 500, 2 ** 30 + 500), slice(n - 20000, n)]
+    g = torch.Generator(device="cuda").manual_seed(d)
+    for r in runs:
+        x[r] = torch.randn((r.stop - r.start, d), generator=g, device="cuda").half()
+    a = K.quantize(x, d)
+    for r in runs:
+        q, s = quant(f32(x[r]), d)
+        assert np.array_equal(a.x[r].cpu().numpy(), q) and bits_equal(f32(a.scales[r]), s)
+    del x, a
+    torch.cuda.empty_cache()
+
+
 def test_other_stream_and_graph(K):
     g = torch.rand(1024, device="cuda") + 0.5
     x = torch.randn((64, 1024), device="cuda", dtype=torch.float16)

@@ -77,10 +77,10 @@ __global__ void __launch_bounds__(MAX_THREADS) rms_quant_kernel(const Params p) 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const bool one_warp = blockDim.y > 1;  // a row per warp, blockDim = (32, WARP_ROWS)
   const int threads = blockDim.x, nwarps = threads >> 5, ng = p.d / p.group;
-  const int step = gridDim.x * blockDim.y;
+  const unsigned step = gridDim.x * blockDim.y, n = p.n;  // rows of up to 2^31 - 1 plus a step pass 31 bits, not 32
   const bool res = NORM && p.v != nullptr;
   Raw<DT> xr[NV], vr[NORM ? NV : 1];
-  auto fetch = [&](int row) {
+  auto fetch = [&](unsigned row) {
     const T* x = static_cast<const T*>(p.x) + (long long)row * p.ld_x;
     const T* v = static_cast<const T*>(p.v) + (long long)row * p.ld_v;
 #pragma unroll
@@ -93,10 +93,10 @@ __global__ void __launch_bounds__(MAX_THREADS) rms_quant_kernel(const Params p) 
       }
     }
   };
-  int row = blockIdx.x * blockDim.y + threadIdx.y;
-  if (VEC && row < p.n) fetch(row);
+  unsigned row = blockIdx.x * blockDim.y + threadIdx.y;
+  if (VEC && row < n) fetch(row);
   // a whole warp, or the whole block where barriers follow, leaves the loop together
-  for (int turn = 0; row < p.n; row += step, turn ^= 1) {
+  for (int turn = 0; row < n; row += step, turn ^= 1) {
     float h[NV][8];
 #pragma unroll
     for (int j = 0; j < NV; j++) {
@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(MAX_THREADS) rms_quant_kernel(const Params p) 
         }
       }
     }
-    if (VEC && row + step < p.n) fetch(row + step);
+    if (VEC && row + step < n) fetch(row + step);
     if (NORM) {
       double sum = 0.0;
 #pragma unroll
@@ -333,7 +333,7 @@ static vxg_status run(Params p, int dtype, bool norm, cudaStream_t st) {
   dim3 block(threads), grid(p.n);
   if (threads == 32) {
     block.y = WARP_ROWS;
-    grid.x = (p.n + WARP_ROWS - 1) / WARP_ROWS;
+    grid.x = ((unsigned)p.n + WARP_ROWS - 1) / WARP_ROWS;
   }
   const size_t smem = p.group < p.d && !p.lanes ? (size_t)block.y * (p.d / p.group) * sizeof(float) : 0;  // <= 16 KB
   with_dtype(dtype, [&](auto tag) {
