@@ -374,6 +374,36 @@ def test_offsets_past_32_bits(KvCache):
     _ok()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hd,heads,new", [(64, 2, 3), (128, 2, 7), (64, 2, 20), (128, 2, 100)])
+def test_longest_sequence(KvCache, hd, heads, new, dtype):
+    """A sequence at the longest length that a table may hold, 2^31 - 256: its last pages are written, read and, through a
+    window, attended to by tiles of every size. The entries in front of those pages are no valid ids."""
+    page, window, last = 128, 500, 8
+    width = 0x7FFFFF00 // page
+    L, near = width * page, last * page  # the same places of the same pages in a short sequence
+    rng = np.random.default_rng(hd + new)
+    ref, c = _pair(KvCache, rng, last, 1, page, hd)
+    for w, s in ((0, c.ks), (1, c.vs)):
+        ref.scales[w] *= np.float32(0.02)
+        s.copy_(torch.from_numpy(ref.scales[w]))
+    table = torch.full((1, width), -1, dtype=torch.int32, device="cuda")
+    table[0, -last:] = torch.arange(last, device="cuda", dtype=torch.int32)
+    short, cu = np.arange(last)[None], [0, new]
+    k, v = _kv(rng, new, 1, hd, dtype)
+    c.write(k, v, table, _int([L - new]), _int(cu))
+    ref.write([f32(k), f32(v)], short, [near - new], cu)
+    _same(ref, c)
+    got = c.read(table, _int([L - 300]), _int([0, 300]), 300)
+    for w in range(2):
+        assert bits_equal(f32(got[w]), ref.rows(w, short, 0, near - 300, near))
+    q = torch.from_numpy(rng.standard_normal((new, heads, hd)).astype(np.float32) * 1.5).to(dtype).cuda()
+    got = f32(c.attend(q, table, _int([L]), _int(cu), scale=0.11, window=window)).astype(np.float64)
+    want, bound = attend(ref, f32(q), short, [near], cu, float(np.float32(0.11)), True, window, dtype)
+    _ok()
+    assert (np.abs(got - want) <= bound).all()
+
+
 def test_a_decoder_step_of_all_operators(KvCache):
     """norm -> q|k|v product -> cache -> attention -> output product onto the residual -> norm -> feed-forward: a prefill
     of two ragged sequences and two captured single-token steps, each operator against its formula on the library's own

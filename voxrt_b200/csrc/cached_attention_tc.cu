@@ -156,14 +156,14 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (x.b == 0) {  // the piece's largest value scale
         const int k0 = ::max(key0, t.kmin), k1 = ::min(key0 + x.nb * BK, t.kmax);
         ref = 0.0f;
-        for (int pg = (k0 >> PL) + lane; pg << PL < k1; pg += 32) {
+        for (int pg = (k0 >> PL) + lane; pg <= (k1 - 1) >> PL; pg += 32) {  // in pages: k1 + 32 pages may pass 31 bits
           const int id = page_id(pg);
           if (id >= 0) ref = fmaxf(ref, __ldg(p.c.v_scales + (size_t)id * KV + h));
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, o));
       }
-      const int pg = (key0 + 16 * lane) >> PL;
+      const int pg = (key0 + 16 * ::min(lane, CHUNKS - 1)) >> PL;
       if (lane < CHUNKS && pg << PL < t.kmax && (pg + 1) << PL > t.kmin) {  // a page that some row sees
         pid = page_id(pg);
         if (pid >= 0) {
