@@ -6,7 +6,7 @@ import torch
 
 from voxrt_b200 import _lib
 from voxrt_b200.cache import KvCache, _Desc
-from voxrt_b200.kernels import Epilogue, Int8Matrix, quantize, rms_quant
+from voxrt_b200.kernels import Epilogue, Int8Matrix, dequantize, gemm_i8, quantize, rms_quant
 
 P = 1 << 20  # stands for a device address: no refused or empty call follows it
 ARG, UNSUP, OK = _lib.VXG_ERR_ARG, _lib.VXG_ERR_UNSUPPORTED, _lib.VXG_OK
@@ -115,3 +115,25 @@ def test_python_refusals():
     with pytest.raises(ValueError, match="int8"):
         KvCache(x, x, x, x)
     assert Epilogue.AddScaled(2.0).kind == 2
+
+
+class _Act:
+    """A QuantAct whose tensors may lie on the CPU."""
+
+    def __init__(self, n, inp, scales, group):
+        self.x, self.scales, self.group, self.n, self.inp = torch.zeros((n, inp), dtype=torch.int8), scales, group, n, inp
+
+
+@pytest.mark.parametrize("shape,group", [((1, 1), 64), ((3, 1), 64), ((4, 3), 16), ((16,), 15), ((5, 1), 64), ((0, 1), 64), ((4, 1), 0)])
+def test_scales_that_do_not_fit_the_codes(shape, group):
+    """Too few scales (left over from a slice, or meant to be broadcast) would be read past their end."""
+    a = _Act(4, 64, torch.ones(shape), group)
+    with pytest.raises(ValueError, match="scales for 4 rows"):
+        dequantize(a)
+    w = _Act(8, 64, None, 64)
+    w.w, w.scales, w.out = w.x, torch.ones(8), 8
+    with pytest.raises(ValueError, match="scales for 4 rows"):
+        gemm_i8(w, a, torch.zeros((4, 8)))
+    for op in (lambda x: dequantize(x), lambda x: gemm_i8(w, x, torch.zeros((4, 8)))):  # the right count goes on
+        with pytest.raises(ValueError, match="CUDA"):
+            op(_Act(4, 64, torch.ones((4, 1)), 64))

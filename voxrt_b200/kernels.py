@@ -243,9 +243,16 @@ def quantize(x: torch.Tensor, group: int = GROUP, stream=None) -> QuantAct:
     return QuantAct(q, s, group)
 
 
+def _scales_of(x: QuantAct) -> torch.Tensor:
+    """x's scales, one for each of its groups: the kernels read that many."""
+    if x.group <= 0 or x.inp % x.group != 0 or x.scales.numel() != x.n * (x.inp // x.group):
+        raise ValueError(f"{x.scales.numel()} scales for {x.n} rows of width {x.inp} in groups of {x.group}")
+    return x.scales
+
+
 def dequantize(x: QuantAct, dtype: torch.dtype = torch.float32, stream=None) -> torch.Tensor:
     """The values that the codes stand for, q * scale, rounded once to `dtype`."""
-    q, s = x.x, x.scales
+    q, s = x.x, _scales_of(x)
     idx = _gpu(stream, q, s)
     if dtype not in _DTYPES:
         raise ValueError(f"element type {dtype} is none of float16, bfloat16, float32")
@@ -326,7 +333,7 @@ def gemm_i8(w: Int8Matrix, x: QuantAct, y: torch.Tensor, bias: torch.Tensor | No
             ep: Epilogue = Epilogue.Store, stream=None) -> torch.Tensor:
     """y[n, out] = epilogue(x w^T + bias) for int8 activations with one scale a token: exact int32 sums, then
     sum * (token scale * channel scale). y: f32, f16 or bf16 rows of any stride, read first for AddScaled."""
-    wq, xq, sx = w.w, x.x, x.scales
+    wq, xq, sx = w.w, x.x, _scales_of(x)
     idx = _gpu(stream, wq, xq, sx, y, bias)
     n, out, inp = x.n, w.out, w.inp
     if x.inp != inp or x.group != inp:
