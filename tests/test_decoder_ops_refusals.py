@@ -137,3 +137,28 @@ def test_scales_that_do_not_fit_the_codes(shape, group):
     for op in (lambda x: dequantize(x), lambda x: gemm_i8(w, x, torch.zeros((4, 8)))):  # the right count goes on
         with pytest.raises(ValueError, match="CUDA"):
             op(_Act(4, 64, torch.ones((4, 1)), 64))
+
+
+def test_quantize_rows_of_an_empty_batch():
+    L = _lib.lib()
+    assert L.vxg_quantize_rows(None, 0, 64, 64, None, None, None) == OK
+    for a in ((None, 4, 64, 64, P, P), (P, 4, 64, 64, None, P), (P, 4, 64, 64, P, None), (P, -1, 64, 64, P, P),
+              (P, 4, 64, 48, P, P), (P, 4, 64, 0, P, P), (None, 0, 0, 1, None, None), (P, 4, 8200, 8200, P, P)):
+        assert L.vxg_quantize_rows(*a, None) == ARG
+
+
+@pytest.mark.parametrize("dtype,pad", [(torch.float32, 0), (torch.float32, 8), (torch.bfloat16, 0)])
+def test_quantize_goes_to_the_operands_gpu(monkeypatch, dtype, pad):
+    """Whatever the type and stride: the call is made on the operand's GPU and the given stream, with x in use there, and
+    the outputs are allocated for that stream."""
+    from voxrt_b200 import kernels as K
+
+    seen = []
+    monkeypatch.setattr(K, "_gpu", lambda stream, *t: 1)
+    monkeypatch.setattr(K, "_like", lambda t, shape, dt, stream: seen.append(stream) or torch.empty(shape, dtype=dt))
+    monkeypatch.setattr(K, "_call", lambda fn, idx, stream, used, *a: seen.append((idx, stream, used[0])))
+    monkeypatch.setattr(K, "QuantAct", lambda *a: a)
+    x = torch.zeros((4, 64 + pad), dtype=dtype)[:, :64]
+    q, s, group = K.quantize(x, 32, stream="side")
+    assert seen[:2] == ["side", "side"] and seen[2][:2] == (1, "side") and seen[2][2] is x
+    assert q.shape == (4, 64) and s.shape == (4, 2) and group == 32

@@ -144,6 +144,31 @@ def test_feeds_the_ternary_product(K, oracle_lib):
     assert bits_equal(f32(y), oracle_lib.gemm(w_rows, sw, q, s, 128))
 
 
+@pytest.mark.parametrize("dtype,pad", [(torch.float32, 0), (torch.float32, 8), (torch.float16, 0)])
+def test_quantize_empty_batch_and_side_stream(K, dtype, pad):
+    """An empty batch gives empty codes; on a side stream, neither the input nor the outputs are handed out again while that
+    stream still has the call in front of it."""
+    wide = lambda n: torch.ones((n, 256 + pad), dtype=dtype, device="cuda")[:, :256]
+    e = K.quantize(wide(0), 128)
+    assert tuple(e.x.shape) == (0, 256) and tuple(e.scales.shape) == (0, 2)
+    side = torch.cuda.Stream()
+    x = wide(1 << 12)
+    want = K.quantize(x, 128)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)
+    a = K.quantize(x, 128, stream=side)
+    old = x.data_ptr()
+    del x
+    again = wide(1 << 12)
+    assert again.data_ptr() != old  # still read by the side stream
+    side.synchronize()
+    assert torch.equal(a.x, want.x) and torch.equal(a.scales, want.scales)
+    codes = a.x.data_ptr()
+    del a
+    assert torch.empty((1 << 12, 256), dtype=torch.int8, device="cuda").data_ptr() != codes  # the side stream's memory
+
+
 @pytest.mark.parametrize("d", [1, 8])  # element by element, and with the next row's look-ahead
 def test_most_rows(K, d):
     """2^31 - 1 rows: the row index plus a step of the grid passes 31 bits. Only a few runs of the input are written, and

@@ -335,7 +335,9 @@ vxg_status vxg_ln_quant(const float* x, int n, int d, const float* g0, const flo
 
 vxg_status vxg_quantize_rows(const float* x, int n, int inp, int group, int8_t* q, float* scales, void* stream) {
   clear_error();
-  VXG_ARG(q && scales, "NULL output");
+  VXG_ARG(n == 0 || (q && scales), "NULL output");
+  VXG_ARG(inp > 0 && group > 0 && inp % group == 0, "group must divide inp");
+  if (n == 0) return VXG_OK;
   return vxg_ln_quant(x, n, inp, nullptr, nullptr, nullptr, nullptr, nullptr, group, q, scales, stream);
 }
 

@@ -225,13 +225,6 @@ def gemm(w: TernaryMatrix, x: QuantAct, y: torch.Tensor, bias: torch.Tensor | No
 def quantize(x: torch.Tensor, group: int = GROUP, stream=None) -> QuantAct:
     """QuantAct::quantize (packed.rs:302-312) on the GPU: per-(token, group) absmax/127 int8. f32, f16 or bf16 rows (any
     row stride); group = x.shape[1] gives the one scale a token that gemm_i8 reads."""
-    if x.dtype == torch.float32 and x.is_contiguous() and x.dim() == 2 and x.shape[1] <= 8192:
-        assert x.is_cuda
-        n, inp = x.shape
-        q = torch.empty((n, inp), dtype=torch.int8, device=x.device)
-        s = torch.empty((n, inp // group), dtype=torch.float32, device=x.device)
-        check(lib().vxg_quantize_rows(_ptr(x), n, inp, group, _ptr(q), _ptr(s), _stream_ptr(stream)))
-        return QuantAct(q, s, group)
     idx = _gpu(stream, x)
     if x.dim() != 2 or x.shape[1] == 0 or group <= 0:
         raise ValueError("quantize takes rows")
@@ -239,7 +232,10 @@ def quantize(x: torch.Tensor, group: int = GROUP, stream=None) -> QuantAct:
     dt, ld = _dt(x), _rows(x, n, d, "x")
     q = _like(x, (n, d), torch.int8, stream)
     s = _like(x, (n, d // group), torch.float32, stream)
-    _call(lib().vxg_quantize_tokens, idx, stream, (x,), x.data_ptr(), ld, dt, n, d, group, q.data_ptr(), s.data_ptr())
+    if x.dtype == torch.float32 and x.is_contiguous() and d <= 8192:
+        _call(lib().vxg_quantize_rows, idx, stream, (x,), x.data_ptr(), n, d, group, q.data_ptr(), s.data_ptr())
+    else:
+        _call(lib().vxg_quantize_tokens, idx, stream, (x,), x.data_ptr(), ld, dt, n, d, group, q.data_ptr(), s.data_ptr())
     return QuantAct(q, s, group)
 
 
