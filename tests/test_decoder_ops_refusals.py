@@ -1,5 +1,8 @@
 """CPU: what the int8 decoder entries refuse, before anything reaches a GPU, and what they accept as empty."""
 import ctypes as C
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -162,3 +165,31 @@ def test_quantize_goes_to_the_operands_gpu(monkeypatch, dtype, pad):
     q, s, group = K.quantize(x, 32, stream="side")
     assert seen[:2] == ["side", "side"] and seen[2][:2] == (1, "side") and seen[2][2] is x
     assert q.shape == (4, 64) and s.shape == (4, 2) and group == 32
+
+
+NO_GPU = """
+from voxrt_b200 import _lib
+from voxrt_b200.cache import _Desc
+import ctypes as C
+L, P = _lib.lib(), 1 << 20
+c = _Desc(P, P, P, P, 8, 2, 16, 64)
+for m in (1, 40, 65, 5000):
+    assert L.vxg_gemm_i8(P, P, P, P, m, 32, 64, 0, 0.0, None, 2, P, 32, None) not in (0, 5) and L.vxg_last_error()
+for n in (1, 5000):
+    assert L.vxg_rms_quant(P, 64, None, 64, 1.0, 2, n, 64, P, 1e-6, None, 64, None, 64, 64, P, P, None) == 2
+    assert L.vxg_quantize_tokens(P, 64, 2, n, 64, 64, P, P, None) == 2
+    assert L.vxg_dequantize_rows(P, P, n, 64, 64, 2, P, None) == 2
+    for dt in range(3):
+        assert L.vxg_cache_attention(C.addressof(c), P, 256, 4, dt, n, P, 1, 4, P, P, 0.1, 1, 0, P, 256, P, 1 << 40, None) != 0
+        assert L.vxg_cache_write(C.addressof(c), P, 128, P, 128, dt, n, P, 1, 4, P, P, None) != 0
+        assert L.vxg_cache_read(C.addressof(c), P, 1, 4, P, P, n, dt, P, P, None) != 0
+    assert L.vxg_cache_attention_workspace_bytes(n, 1, 4, 2, 64, 2) > 0
+"""
+
+
+def test_without_a_gpu():
+    """A process that sees no GPU gets errors from every entry, and lives on."""
+    env = {**os.environ, "CUDA_VISIBLE_DEVICES": ""}
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", NO_GPU], cwd=root, env=env, capture_output=True, text=True)
+    assert r.returncode == 0, (r.returncode, r.stderr[-800:])

@@ -416,7 +416,7 @@ vxg_status launch(const Params& p, cudaStream_t st) {
 
 // Channels of a tile: rounds of tiles over the pairs of SMs times a stage's time, which was measured as 0.29, 0.39 and 0.72 us
 // per 256 k for 64, 128 and 256 channels: near bn + 64.
-static int pick_bn(const Params& p, int pairs) {
+static int pick_bn(const Params& p, int pairs) {  // pairs > 0
   int best = 256;
   long long cost = 0;
   for (int bn = 256; bn >= 64; bn /= 2) {
@@ -463,7 +463,7 @@ extern "C" vxg_status vxg_gemm_i8(const int8_t* x, const float* sx, const int8_t
         default: r = i8::launch_few<DT, 8>(p, st); break;
       }
     } else {
-      const int bn = i8::pick_bn(p, sm_count() / 2);
+      const int bn = i8::pick_bn(p, std::max(1, sm_count() / 2));  // no GPU: the launch says so
       r = bn == 256 ? i8::tc::launch<DT, 256>(p, st)
           : bn == 128 ? i8::tc::launch<DT, 128>(p, st) : i8::tc::launch<DT, 64>(p, st);
     }
