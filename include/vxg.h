@@ -155,7 +155,7 @@ vxg_status vxg_dequantize_rows(const int8_t* q, const float* scales, int n, int 
  * y[t, o] = ep(f32(sum_k x[t, k] w[o, k]) * (sx[t] * sw[o]) (+ bias[o])) for t < M, o < N, the sum exact in int32: one
  * scale a token, one an output channel. x [M, K] and w [N, K] int8 (device, contiguous, 16-byte aligned), sx [M],
  * sw [N], bias [N] or NULL (f32), y rows of `dtype` elements with stride ld_y >= N (read first for ADD_SCALED:
- * y = fma(ep_scale, v, y)). K a multiple of 16 below 131072 (else VXG_ERR_UNSUPPORTED); codes of -128 are allowed. The
+ * y = fma(ep_scale, v, y)). K a multiple of 16 below 131072, M and N up to 2^31 - 256 (else VXG_ERR_UNSUPPORTED); codes of -128 are allowed. The
  * same bits for every M: a token's row does not depend on the batch it is computed in. Stands beside
  * vxg_gemm_ternary_i8 for weights that are not ternary; no reference counterpart. */
 vxg_status vxg_gemm_i8(const int8_t* x, const float* sx, const int8_t* w, const float* sw, int M, int N, int K,

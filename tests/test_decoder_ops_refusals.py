@@ -127,6 +127,12 @@ class _Act:
         self.x, self.scales, self.group, self.n, self.inp = torch.zeros((n, inp), dtype=torch.int8), scales, group, n, inp
 
 
+@pytest.mark.parametrize("kw", [dict(m=0x7FFFFFFF), dict(m=0x7FFFFF01), dict(n=0x7FFFFFFF, ld=0x7FFFFFFF),
+                                dict(m=1, n=0x7FFFFF01, ld=0x7FFFFF01)])
+def test_gemm_sizes_that_pass_31_bits_within_a_tile(kw):
+    test_gemm(kw, UNSUP)
+
+
 @pytest.mark.parametrize("shape,group", [((1, 1), 64), ((3, 1), 64), ((4, 3), 16), ((16,), 15), ((5, 1), 64), ((0, 1), 64), ((4, 1), 0)])
 def test_scales_that_do_not_fit_the_codes(shape, group):
     """Too few scales (left over from a slice, or meant to be broadcast) would be read past their end."""

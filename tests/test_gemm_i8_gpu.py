@@ -82,6 +82,27 @@ def test_extreme_codes(K):
         assert torch.equal(y.cpu(), want.expand(m, 130))
 
 
+def test_most_tokens(K):
+    """As many tokens as the entry takes, 2^31 - 256. Only a few runs of the input are written, and compared."""
+    m, k = 2 ** 31 - 256, 16
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < m * 22 * 1.2:
+        pytest.skip("not enough memory")
+    x = torch.empty((m, k), dtype=torch.int8, device="cuda")
+    sx, y = torch.empty((m, 1), device="cuda"), torch.empty((m, 1), dtype=torch.float16, device="cuda")
+    runs = [slice(0, 600), slice(2 ** 30 - 300, 2 ** 30 + 300), slice(m - 600, m)]
+    parts = [_case(i, 600, 1, k) for i in range(len(runs))]
+    _, _, w, sw, _, _ = parts[0]
+    for r, p in zip(runs, parts):
+        x[r], sx[r] = p[0], p[1]
+    K.gemm_i8(K.Int8Matrix(w, sw), K.QuantAct(x, sx, k), y)
+    for r, p in zip(runs, parts):
+        s = (p[0].double() @ w.double().t()).float() * (p[1] * sw[None])
+        assert torch.equal(y[r], s.half())
+    del x, sx, y
+    torch.cuda.empty_cache()
+
+
 def test_rows_do_not_depend_on_the_batch(K):
     x, sx, w, sw, _, v = _case(11, 700, 384, 1024)
     W = K.Int8Matrix(w, sw)

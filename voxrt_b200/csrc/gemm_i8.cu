@@ -446,6 +446,10 @@ extern "C" vxg_status vxg_gemm_i8(const int8_t* x, const float* sx, const int8_t
     set_error("K = %d not supported (a multiple of 16 below 131072)", K);
     return VXG_ERR_UNSUPPORTED;
   }
+  if (M > 0x7FFFFF00 || N > 0x7FFFFF00) {  // rows and channels of the last tile are counted in 31 bits
+    set_error("M = %d x N = %d not supported (up to 2^31 - 256 each)", M, N);
+    return VXG_ERR_UNSUPPORTED;
+  }
   if (M == 0) return VXG_OK;
   i8::Params p = {x, sx, w, sw, bias, y, ld_y, M, N, K, (int)ep, ep_scale};
   vxg_status r = VXG_OK;
