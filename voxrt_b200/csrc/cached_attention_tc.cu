@@ -91,7 +91,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   float* ref_s = reinterpret_cast<float*>(smem + Lay::REF);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Lay::BARS);
   uint64_t *kfull = bars, *kempty = bars + 2, *vfull = bars + 4, *vempty = bars + 6;  // by stage
-  uint64_t *qfull = bars + 8, *sfull = bars + 10, *pfull = bars + 14, *odone = bars + 18;  // by half; sfull, pfull: and buffer
+  uint64_t *qfull = bars + 8, *sfull = bars + 10, *pfull = bars + 14;  // by half; sfull, pfull: and buffer
+  uint64_t* obut = bars + 18;  // by half: a piece's products but the last step's
   uint64_t* drain = bars + 20;
   uint64_t *rkfull = bars + 21, *rkempty = bars + 22, *rvfull = bars + 23, *rvempty = bars + 24;
   uint64_t* ofull = bars + 25;  // by half: the last product of a piece
@@ -107,7 +108,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(vfull + i, CONV_WARPS);
       mbar_init(vempty + i, 1);
       mbar_init(qfull + i, 4);
-      mbar_init(odone + i, 1);
+      mbar_init(obut + i, 1);
       mbar_init(ofull + i, 1);
     }
     for (int i = 0; i < 4; i++) {
@@ -297,14 +298,13 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       __syncwarp();
     };
-    auto values = [&](int half, uint32_t n, int st, int sub, bool fresh, bool last) {
+    auto values = [&](int half, uint32_t n, int st, int sub, bool fresh, int left) {  // left: steps of the piece behind this
       const uint64_t v = desc_mn + (Lay::V + st * Lay::OPER + sub * SB * 128) / 16;
       if (leader) {
 #pragma unroll
         for (int j = 0; j < SB / 16; j++)
           mma_f16_ts(tmem + 256 + half * HD, tmem + half * 128 + (n & 1) * SB + 8 * j, v + j * 128, PV, fresh && j == 0 ? 0u : 1u);
-        mma_commit(odone + half);
-        if (last) mma_commit(ofull + half);
+        if (left <= 1) mma_commit((left == 1 ? obut : ofull) + half);
       }
       __syncwarp();
     };
@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const bool more = i + 2 < ns;
         if (sub == 0 && !wait(vfull + st, it >> 1)) break;
         if (!wait(pfull + (n0 & 1), n0 >> 1)) break;
-        values(0, n0, st, sub, i == 0, i + 1 == ns);
+        values(0, n0, st, sub, i == 0, ns - 1 - i);
         if (more) {  // the step after next, over the probabilities that these products read
           if (sub == 0 && !wait(kfull + (st ^ 1), (it + 1) >> 1)) break;
           scores(0, n0 + 2, st ^ 1, sub);
@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         n0++;
         if (two) {
           if (!wait(pfull + 2 + (n1 & 1), n1 >> 1)) break;
-          values(1, n1, st, sub, i == 0, i + 1 == ns);
+          values(1, n1, st, sub, i == 0, ns - 1 - i);
           if (more) scores(1, n1 + 2, st ^ 1, sub);
           n1++;
         }
@@ -469,8 +469,10 @@ __global__ void __launch_bounds__(THREADS, 1)
             const float alpha = grow ? ex2(m - mx) : 1.0f;
             if (grow) m = mx;
             l *= alpha;
-            if (b > 0) {  // once the products of the step before are in O (those before them are, or these scores were not)
-              if (!wait_phase(odone + half, (it - 1) & 1, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN)) ok = false;
+            if (b > 0) {  // once the products of the step before are in O: the next step's scores come behind them
+              const bool more = b + 1 < 2 * nb;
+              uint64_t* bar = more ? sfull + 2 * half + (buf ^ 1) : obut + half;
+              if (!wait_phase(bar, (more ? (it + 1) >> 1 : pieces) & 1, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN)) ok = false;
               ok = __all_sync(0xffffffffu, ok);
               if (!ok) break;
               tc_fence_after();
@@ -534,7 +536,9 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (lane == 0) mbar_arrive(pfull + 2 * half + buf);
         }
         ring += nb;
-        // a barrier of its own: when a warp comes here, odone may be one or two phases behind
+        // Every phase of every barrier is met once and in turn, obut's too where no reference has moved in the last step: a
+        // wait by parity is right only if the phase before was met, and commits to two barriers have no order that PTX states.
+        if (ok && !wait_phase(obut + half, pieces & 1, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN)) ok = false;
         if (ok && !wait_phase(ofull + half, pieces & 1, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN)) ok = false;
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
