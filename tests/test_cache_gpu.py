@@ -299,6 +299,29 @@ def test_scales_that_are_not_positive(KvCache, hd, heads, new, dtype, scale):
     assert (np.abs(got - want) <= bound).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("length", [257, 300, 448, 1000])  # the last step of 64 keys: one key, a few, none, most
+@pytest.mark.parametrize("hd,heads,new", [(64, 2, 3), (128, 2, 7), (64, 2, 30), (128, 2, 30), (64, 2, 150), (128, 2, 150)])
+def test_scores_that_rise_all_along(KvCache, hd, heads, new, length, dtype):
+    """Every 64 keys outweigh all before them by about e^7.6, so that the softmax's reference moves in every step, in
+    tiles of every size."""
+    rng = np.random.default_rng(hd + new + length)
+    table, n_pages = _table(rng, [length], 16)
+    ref, c = _pair(KvCache, rng, n_pages, 1, 16, hd)
+    sign = np.where(rng.random(hd) < 0.5, -1, 1)
+    for pg in range(-(-length // 16)):  # scores: about 1.9 a page on
+        ref.codes[0][table[0, pg], 0] = sign[None] * rng.integers(112, 128, (16, 1))
+        ref.scales[0][table[0, pg]] = np.float32((pg + 1) * 2.0 / 127 / hd)
+    c.k.copy_(torch.from_numpy(ref.codes[0]))
+    c.ks.copy_(torch.from_numpy(ref.scales[0]))
+    q = torch.from_numpy(np.tile(sign, (new, heads, 1)).astype(np.float32)).to(dtype).cuda()
+    cu = [0, new]
+    got = f32(c.attend(q, _int(table), _int([length]), _int(cu), scale=1.0)).astype(np.float64)
+    want, bound = attend(ref, f32(q), table, [length], cu, 1.0, True, 0, dtype)
+    _ok()
+    assert (np.abs(got - want) <= bound).all()
+
+
 def test_shared_pages_other_stream_and_graph(KvCache):
     """Two sequences over the same prefix pages; a captured call replayed with other lengths; a side stream."""
     rng = np.random.default_rng(10)
