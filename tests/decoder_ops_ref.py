@@ -82,8 +82,8 @@ class Cache:
         return out
 
 
-def attend(cache, q, table, lens, cu, scale, causal, window, dtype):
-    """(out, bound) in 64 bits; `bound` is how far the library's result may be off, element by element.
+def attend(cache, q, table, lens, cu, scale, causal, window, dtype, hidden=()):
+    """(out, bound) in 64 bits, without the keys of the pages hidden (sequence, place in its table); `bound` is how far the library's result may be off, element by element.
 
     Per probability: f16 rounding, 11 significant bits and so at most 2^-11 (f32 queries: two parts, 2^-22), and the error of
     its score, twice (numerator and denominator). Codes are exact, and the value scales enter in f32 before that rounding. A score is a sum of hd exact products in f32, in the tensor cores' order: at most (hd + 8) half-steps
@@ -110,6 +110,9 @@ def attend(cache, q, table, lens, cu, scale, causal, window, dtype):
                 seen &= np.arange(L) <= pos
             if window:
                 seen &= np.arange(L) > pos - window
+            for hs, pg in hidden:
+                if hs == s:
+                    seen[pg * cache.page:(pg + 1) * cache.page] = False
             if not seen.any():
                 continue
             biased = 0.0

@@ -159,6 +159,34 @@ def test_bad_indices_are_skipped_and_reported(KvCache):
     assert device_status() == 0x302 and (out[1:] == 3.0).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("page", [16, 128])
+@pytest.mark.parametrize("hd,heads,new", [(64, 2, 3), (128, 2, 7), (64, 2, 30), (128, 2, 30), (64, 2, 150), (128, 2, 150)])
+def test_pages_out_of_range_are_masked(KvCache, hd, heads, new, page, dtype):
+    """The keys of a page whose id is out of range take no part, in tiles of every size: first, middle and last pages, a
+    sequence that has no other, and one that is sound."""
+    from voxrt_b200._lib import device_status
+
+    rng = np.random.default_rng(hd + new + page)
+    lens = [5 * page + 7, 2 * page, page + 1, 700]
+    table, n_pages = _table(rng, lens, page)
+    ref, c = _pair(KvCache, rng, n_pages, 1, page, hd)
+    ref.scales[0] *= np.float32(0.02)
+    c.ks.copy_(torch.from_numpy(ref.scales[0]))
+    hidden = [(0, 0), (0, 2), (0, 5), (1, 0), (1, 1), (2, 1)]
+    bad = table.copy()
+    for i, (s, pg) in enumerate(hidden):
+        bad[s, pg] = [-1, n_pages, 1 << 30][i % 3]
+    count = [min(new, 5 * page), min(new, page), 1, new]
+    cu = np.concatenate([[0], np.cumsum(count)])
+    q = torch.from_numpy(rng.standard_normal((int(cu[-1]), heads, hd)).astype(np.float32) * 1.5).to(dtype).cuda()
+    for window in (0, page + 3):
+        got = f32(c.attend(q, _int(bad), _int(lens), _int(cu), scale=0.11, window=window)).astype(np.float64)
+        want, bound = attend(ref, f32(q), table, lens, cu, float(np.float32(0.11)), True, window, dtype, hidden)
+        assert device_status() == 0x302
+        assert (np.abs(got - want) <= bound).all()
+
+
 CASES = [  # (page, hd, kv heads, query heads, lengths, new tokens, causal, window)
     (16, 64, 1, 1, [1], [1], True, 0),
     (16, 64, 2, 2, [1, 17, 64, 65, 200], [1, 1, 1, 1, 1], True, 0),

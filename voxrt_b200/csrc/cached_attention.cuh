@@ -36,6 +36,9 @@ struct Plan {
   size_t rec_bytes, part_bytes;
 };
 
+// Stands for the key scale of a page whose id is out of range: its keys take no part. A written page's is not negative.
+constexpr float NO_PAGE = -1.0f;
+
 constexpr int FEW_CTAS_8 = 3;  // CTAs an SM, tiles of up to 8 rows
 // Tiles of up to 16 rows (cached_attention_few.cu).
 vxg_status launch_few(const Params& p, const Plan& pl, int head_dim, int dtype, cudaStream_t st);
@@ -190,7 +193,8 @@ __device__ __forceinline__ void find_share(const Params& p, Piece* first_s) {
 
 // One warp brings the share's blocks of BK keys: codes [K BK x HD][V BK x HD] by TMA, one box per page, into a ring of
 // STAGES stages, and the scales of a block's 16-key pieces (four of K, four of V) beside it. Pages and scales are looked
-// up 32 pages at a time. Pages that no row of the tile sees are not brought and have scale 0.
+// up 32 pages at a time. Pages that no row of the tile sees are not brought and have scale 0; a page whose id is out of range
+// is not brought either, and has key scale NO_PAGE.
 template <int HD, int MT, int BK, int STAGES>
 __device__ __forceinline__ void produce(const Params& p, Piece w, const CUtensorMap& map_k, const CUtensorMap& map_v,
                                         uint8_t* smem, float* scales_s, uint64_t* full, uint64_t* empty) {
@@ -216,6 +220,7 @@ __device__ __forceinline__ void produce(const Params& p, Piece w, const CUtensor
             if (pid < 0 || pid >= p.c.n_pages) {
               atomicCAS(p.status + 1, 0, VXG_DEV_CACHE_INDEX);
               pid = -1;
+              ks = NO_PAGE;
             } else {
               ks = __ldg(p.c.k_scales + (size_t)pid * KV + h);
               vs = __ldg(p.c.v_scales + (size_t)pid * KV + h);

@@ -47,7 +47,7 @@ struct Layout {
   static constexpr uint32_t RK = V + 2 * OPER, RV = RK + RAW;
   static constexpr uint32_t KS = RV + RAW;                // [RING][8] f32: key scales of the block's 16-key pieces
   static constexpr uint32_t VF = KS + RING * 32;          // [RING][8] f32: their value scales / ref
-  static constexpr uint32_t REF = VF + RING * 32;         // [RING] f32
+  static constexpr uint32_t REF = VF + RING * 32;         // [RING] f32, its sign bit set where one of the piece's page ids is out of range
   static constexpr uint32_t BARS = REF + RING * 4;
   static constexpr uint32_t BYTES = BARS + 27 * 8 + 1024;
   static_assert(BYTES <= 232448, "shared memory budget");
@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     // Lane l holds the page and scales of the block's 16-key piece l; a page's first piece brings it.
     constexpr int CHUNKS = BK / 16;
     const int ppp = 1 << (PL - 4), box = ::min(128, 1 << PL);  // pieces of a page, rows of a copy
-    bool ok = true;
+    bool ok = true, gone = false;
     float ref = 0.0f;
     int it = 0;
     for (Blocks x(p, first); !x.done() && ok; x.next(p), it++) {
@@ -157,12 +157,15 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (x.b == 0) {  // the piece's largest value scale
         const int k0 = ::max(key0, t.kmin), k1 = ::min(key0 + x.nb * BK, t.kmax);
         ref = 0.0f;
+        gone = false;
         for (int pg = (k0 >> PL) + lane; pg <= (k1 - 1) >> PL; pg += 32) {  // in pages: k1 + 32 pages may pass 31 bits
           const int id = page_id(pg);
           if (id >= 0) ref = fmaxf(ref, __ldg(p.c.v_scales + (size_t)id * KV + h));
+          else gone = true;
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, o));
+        gone = __any_sync(0xffffffffu, gone);
       }
       const int pg = (key0 + 16 * ::min(lane, CHUNKS - 1)) >> PL;
       if (lane < CHUNKS && pg << PL < t.kmax && (pg + 1) << PL > t.kmin) {  // a page that some row sees
@@ -170,6 +173,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (pid >= 0) {
           ks = __ldg(p.c.k_scales + (size_t)pid * KV + h);
           vs = __ldg(p.c.v_scales + (size_t)pid * KV + h);
+        } else {
+          ks = NO_PAGE;
         }
       }
       const bool bring = pid >= 0 && lane % ppp == 0;
@@ -182,7 +187,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         ks_s[(it % RING) * 8 + lane] = ks;
         vf_s[(it % RING) * 8 + lane] = ref > 0.0f ? vs / ref : 0.0f;
       }
-      if (lane == 8 && x.b == 0) ref_s[x.piece % RING] = ref;
+      if (lane == 8 && x.b == 0) ref_s[x.piece % RING] = gone ? -ref : ref;
       __syncwarp();
       if (lane == 0) mbar_arrive_expect_tx(rkfull, bytes);
       __syncwarp();
@@ -414,7 +419,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                 make_uint4(h[0], h[1], h[2], h[3]);
           }
         }
-        const float rowf = __int_as_float((127 - ex) << 23) * p.scale_log2;
+        // not 0, so that NO_PAGE times infinity is one; below f32's range the scores are alike in any case
+        const float rowf = fmaxf(__int_as_float((127 - ex) << 23) * p.scale_log2, 1.4e-45f);
         fence_proxy_async_smem();
         tc_fence_before();
         __syncwarp();
@@ -434,6 +440,12 @@ __global__ void __launch_bounds__(THREADS, 1)
           const int scales = ((ring + b / 2) % RING) * 8 + (b & 1) * (SB / 16);
           const float *ks = ks_s + scales, *vf = vf_s + scales;
           if (b == 0) ref = ref_s[ring_piece % RING];
+          if (__float_as_int(ref) < 0) {  // scores that NO_PAGE takes to -inf, whatever the query
+#pragma unroll 1
+            for (int g = 0; g < SB / 16; g++)
+              if (ks[g] < 0.0f) tmem_st16_const(S + 16 * g, __float_as_uint(INFINITY));
+            tmem_wait_st();
+          }
           // ---- the step's maximum
           float mx = -INFINITY;
           auto maximum = [&](auto tag) {
@@ -567,7 +579,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             uint32_t h[4];
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-              const float v0 = __uint_as_float(a[j + 2 * k]) * inv * ref, v1 = __uint_as_float(a[j + 2 * k + 1]) * inv * ref;
+              const float v0 = __uint_as_float(a[j + 2 * k]) * inv * fabsf(ref), v1 = __uint_as_float(a[j + 2 * k + 1]) * inv * fabsf(ref);
               h[k] = narrow2<DT>(l == 0.0f ? 0.0f : v0, l == 0.0f ? 0.0f : v1);
             }
             *reinterpret_cast<uint4*>(os + (c / 64) * Lay::HALF +
@@ -578,7 +590,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
           for (int j = 0; j < 32; j += 2)
             *reinterpret_cast<float2*>(part + 2 + c + j) =
-                make_float2(__uint_as_float(a[j]) * ref, __uint_as_float(a[j + 1]) * ref);
+                make_float2(__uint_as_float(a[j]) * fabsf(ref), __uint_as_float(a[j + 1]) * fabsf(ref));
         }
         __syncwarp();
       }
