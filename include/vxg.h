@@ -189,9 +189,9 @@ vxg_status vxg_attention_i8(const float* qkv, int ld_qkv, const float* rel_k, in
  * out (cu: device int32 [n_seq + 1], not decreasing, cu[n_seq] <= total; rows behind the last sequence are neither read
  * nor written). Lengths are device arrays, so calls can be captured in a CUDA graph and replayed with other lengths
  * (make one call before the capture: it allocates the device's status word). A page id, length or offset that is out
- * of range is not followed: its part of the work is skipped and vxg_device_status reports 0x302. (Page ids: their tokens
- * are not written, their rows of a read stay as they are, their keys are masked. Lengths and offsets: so for the whole
- * sequence, whose rows of the output stay as they are.) */
+ * of range is not followed: its part of the work is skipped and vxg_device_status reports 0x302. (A page id: its tokens
+ * are not written, their rows of a read stay as they are, its keys are masked. A length or offset: the whole sequence is
+ * left out, and its rows of an output stay as they are. Offsets that decrease may go unreported.) */
 typedef struct vxg_kv_cache {
   int8_t *k, *v;            /* [n_pages][heads][page][head_dim] */
   float *k_scales, *v_scales; /* [n_pages][heads] */

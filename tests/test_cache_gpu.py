@@ -159,6 +159,29 @@ def test_bad_indices_are_skipped_and_reported(KvCache):
     assert device_status() == 0x302 and (out[1:] == 3.0).all()
 
 
+def test_read_leaves_out_what_is_out_of_range(KvCache):
+    """A sequence whose rows run past the output, or whose positions run past the table, is left out as a whole, as in a
+    write, and reported; the others are read."""
+    from voxrt_b200._lib import check, device_status, lib
+
+    rng = np.random.default_rng(4)
+    table, n_pages = _table(rng, [40, 40], 16)
+    ref, c = _pair(KvCache, rng, n_pages, 2, 16, 64)
+    most = 16 * table.shape[1]
+    for start, cu, sound in (([0, 0], [0, 20, 41], [0]), ([0, most - 10], [0, 20, 40], [0]), ([-1, 3], [0, 20, 40], [1]),
+                             ([5, 7], [0, 20, 40], [0, 1])):
+        out = torch.full((2, 40, 2, 64), 5.0, device="cuda")
+        t, a, o = _int(table), _int(start), _int(cu)
+        check(lib().vxg_cache_read(c._ref, t.data_ptr(), 2, table.shape[1], a.data_ptr(), o.data_ptr(), 40, 2,
+                                   out[0].data_ptr(), out[1].data_ptr(), torch.cuda.current_stream().cuda_stream))
+        assert device_status() == (0 if len(sound) == 2 else 0x302)
+        for w in range(2):
+            for s in range(2):
+                got = f32(out[w][cu[s]:min(cu[s + 1], 40)])
+                want = ref.rows(w, table, s, start[s], start[s] + 20) if s in sound else np.full_like(got, 5.0)
+                assert bits_equal(got, want)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("page", [16, 128])
 @pytest.mark.parametrize("hd,heads,new", [(64, 2, 3), (128, 2, 7), (64, 2, 30), (128, 2, 30), (64, 2, 150), (128, 2, 150)])

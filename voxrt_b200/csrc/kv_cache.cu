@@ -218,12 +218,12 @@ __global__ void __launch_bounds__(256) cache_read_kernel(ReadParams p) {
   const long long tok = i / vpt;
   if (tok >= p.total) return;
   while (lo + 1 < p.n_seq && __ldg(p.cu + lo + 1) <= tok) lo++;
-  const long long a = __ldg(p.start + lo), at = tok - __ldg(p.cu + lo);
-  if (at < 0 || tok >= __ldg(p.cu + lo + 1)) return;  // rows behind the last sequence stay as they are
+  const long long a = __ldg(p.start + lo), t0 = __ldg(p.cu + lo), t1 = __ldg(p.cu + lo + 1), at = tok - t0;
+  if (at < 0 || tok >= t1) return;  // rows behind the last sequence stay as they are
   const int e = (int)(i % vpt) * 16, h = e / D;
   const long long pos = a + at;
   int pid = -1;
-  if (a >= 0 && pos < (long long)p.max_pages * P) pid = __ldg(p.table + (size_t)lo * p.max_pages + pos / P);
+  if (t0 >= 0 && t1 <= p.total && a >= 0 && a + (t1 - t0) <= (long long)p.max_pages * P) pid = __ldg(p.table + (size_t)lo * p.max_pages + pos / P);
   if (pid < 0 || pid >= p.c.n_pages) {
     atomicCAS(p.status + 1, 0, VXG_DEV_CACHE_INDEX);
     return;
