@@ -48,8 +48,8 @@ const char* vxg_last_error(void);
 const char* vxg_version(void);
 
 /* Synchronise the current device, return its device status word in *code (0 = no kernel reported a problem;
- * nonzero = a bounded wait expired, code identifies the role) and clear it. No reference counterpart: the
- * reference's CPU kernels cannot time out. */
+ * 0x302 = a page id, length or offset of a cache call was out of range; other codes = a bounded wait expired, the code
+ * identifies the role) and clear it. No reference counterpart: the reference's CPU kernels cannot time out. */
 vxg_status vxg_device_status(int* code);
 
 /* ---------------------------------------------------------------------------------------- ternary weights

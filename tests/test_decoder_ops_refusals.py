@@ -199,3 +199,13 @@ def test_without_a_gpu():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", NO_GPU], cwd=root, env=env, capture_output=True, text=True)
     assert r.returncode == 0, (r.returncode, r.stderr[-800:])
+
+
+def test_device_status_says_what_happened(monkeypatch):
+    for code, status, text in ((0x302, ARG, "page id, length or offset"), (0x301, _lib.VXG_ERR_TIMEOUT, "bounded wait")):
+        monkeypatch.setattr(_lib, "device_status", lambda: code)
+        with pytest.raises(_lib.VxgError, match=text) as e:
+            _lib.check_device()
+        assert e.value.status == status
+    monkeypatch.setattr(_lib, "device_status", lambda: 0)
+    _lib.check_device()

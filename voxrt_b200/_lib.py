@@ -11,6 +11,8 @@ LIB_PATH = os.path.join(HERE, "libvxg.so")
 VXG_OK, VXG_ERR_ARG, VXG_ERR_CUDA, VXG_ERR_TIMEOUT, VXG_ERR_OOM, VXG_ERR_UNSUPPORTED = range(6)
 STATUS_NAMES = {0: "OK", 1: "ERR_ARG", 2: "ERR_CUDA", 3: "ERR_TIMEOUT", 4: "ERR_OOM", 5: "ERR_UNSUPPORTED"}
 
+DEV_CACHE_INDEX = 0x302  # VXG_DEV_CACHE_INDEX
+
 _P, _I, _F, _Z, _L = C.c_void_p, C.c_int, C.c_float, C.c_size_t, C.c_longlong
 
 # name -> (restype, argtypes): every symbol include/vxg.h declares
@@ -148,5 +150,8 @@ def device_status() -> int:
 
 def check_device():
     code = device_status()
+    if code == DEV_CACHE_INDEX:
+        raise VxgError(VXG_ERR_ARG, f"a kernel reported device status 0x{code:x} (a page id, length or offset of a cache "
+                                    "call was out of range; its part was left out)")
     if code:
         raise VxgError(VXG_ERR_TIMEOUT, f"a kernel reported device status 0x{code:x} (bounded wait expired)")
