@@ -209,3 +209,26 @@ def test_device_status_says_what_happened(monkeypatch):
         assert e.value.status == status
     monkeypatch.setattr(_lib, "device_status", lambda: 0)
     _lib.check_device()
+
+
+def test_operands_across_an_element_boundary():
+    """A pointer that is no multiple of its element would fault on the GPU."""
+    L, c = _lib.lib(), _cache()
+
+    def refused(status):
+        return status == ARG and b"aligned" in L.vxg_last_error()
+
+    for dt, off in ((0, 1), (1, 1), (2, 2)):
+        for kw in (dict(x=P + off), dict(v=P + off), dict(v=P, res=P + off), dict(y=P + off), dict(gamma=P + 2), dict(s=P + 1)):
+            assert refused(_rms(dt=dt, **kw)), kw
+        assert refused(L.vxg_quantize_tokens(P + off, 64, dt, 4, 64, 64, P, P, None))
+        assert refused(L.vxg_dequantize_rows(P, P, 4, 64, 64, dt, P + off, None))
+        for sx, sw, bias, y in ((P + 2, P, None, P), (P, P + 1, None, P), (P, P, P + 2, P), (P, P, None, P + off)):
+            assert refused(L.vxg_gemm_i8(P, sx, P, sw, 4, 32, 64, 0, 0.0, bias, dt, y, 32, None))
+        assert refused(_write(c, dt=dt, k=P + off)) and refused(_write(c, dt=dt, v=P + off))
+    assert refused(L.vxg_dequantize_rows(P, P + 2, 4, 64, 64, 2, P, None))
+    for kw in (dict(table=P + 2), dict(cu=P + 1)):
+        assert refused(_write(c, **kw)) and refused(_attend(c, **kw)) and refused(_read(c, **kw))
+    assert refused(_write(c, start=P + 2)) and refused(_attend(c, lens=P + 2)) and refused(_read(c, start=P + 2))
+    for kw in (dict(k_scales=P + 2), dict(v_scales=P + 1)):
+        assert refused(_write(_cache(**kw))) and refused(_attend(_cache(**kw))) and refused(_read(_cache(**kw)))

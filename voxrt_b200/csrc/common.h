@@ -54,6 +54,12 @@ inline vxg_status cuda_fail(cudaError_t e, const char* what) {
     }                               \
   } while (0)
 
+// Whether every pointer (NULL is) is a multiple of `bytes`, a power of two: an element across its boundary faults.
+template <class... P>
+inline bool aligned(size_t bytes, const P*... p) {
+  return (((uintptr_t)p | ...) & (bytes - 1)) == 0;
+}
+
 // 2D tensor map over a row-major [rows, cols] matrix of 1-byte elements with a (box_rows x box_cols) box and the
 // swizzle of its row: 64 columns take the 64-byte swizzle, 128 the 128-byte one.
 vxg_status make_tmap_2d_u8(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t row_stride,

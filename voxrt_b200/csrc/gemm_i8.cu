@@ -441,7 +441,8 @@ extern "C" vxg_status vxg_gemm_i8(const int8_t* x, const float* sx, const int8_t
   VXG_ARG(dtype_known(dtype), "unknown element type %d", dtype);
   VXG_ARG(ep == VXG_EP_STORE || ep == VXG_EP_SILU || ep == VXG_EP_ADD_SCALED, "bad epilogue %d", (int)ep);
   VXG_ARG(ld_y >= N, "output row stride %lld is below N = %d", ld_y, N);
-  VXG_ARG((((uintptr_t)x | (uintptr_t)w) & 15) == 0, "x and w must be 16-byte aligned");
+  VXG_ARG(aligned(16, x, w), "x and w must be 16-byte aligned");
+  VXG_ARG(aligned(4, sx, sw, bias) && aligned(dtype_bytes(dtype), y), "an operand is not aligned to its elements");
   if (K % 16 != 0 || K >= 131072) {
     set_error("K = %d not supported (a multiple of 16 below 131072)", K);
     return VXG_ERR_UNSUPPORTED;

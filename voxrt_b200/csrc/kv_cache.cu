@@ -252,7 +252,8 @@ vxg_status cache_check(const vxg_kv_cache* c) {
   VXG_ARG(c, "NULL cache");
   VXG_ARG(c->n_pages > 0 && c->heads > 0, "bad cache shape: %d pages of %d heads", c->n_pages, c->heads);
   VXG_ARG(c->k && c->v && c->k_scales && c->v_scales, "NULL cache buffer");
-  VXG_ARG((((uintptr_t)c->k | (uintptr_t)c->v) & 15) == 0, "the cache's codes must be 16-byte aligned");
+  VXG_ARG(aligned(16, c->k, c->v) && aligned(4, c->k_scales, c->v_scales),
+          "the cache's codes must be 16-byte aligned, its scales 4-byte aligned");
   if ((c->page != 16 && c->page != 32 && c->page != 64 && c->page != 128) ||
       (c->head_dim != 64 && c->head_dim != 128) || c->heads > 65535 ||
       (long long)c->n_pages * c->heads * c->page > 0x7FFFFFFFLL) {
@@ -268,6 +269,7 @@ vxg_status cache_batch_check(const vxg_kv_cache* c, const int* table, int n_seq,
   VXG_ARG(n_seq >= 0 && max_pages >= 0 && total >= 0, "bad batch: %d sequences of %d pages, %d rows", n_seq, max_pages,
           total);
   VXG_ARG(n_seq == 0 || total == 0 || (table && a && cu && max_pages > 0), "NULL page table, lengths or offsets");
+  VXG_ARG(aligned(4, table, a, cu), "page table, lengths and offsets must be 4-byte aligned");
   if ((long long)max_pages * c->page > 0x7FFFFF00LL) {
     set_error("sequences of %d pages of %d tokens not supported", max_pages, c->page);
     return VXG_ERR_UNSUPPORTED;
@@ -291,6 +293,7 @@ vxg_status vxg_cache_write(const vxg_kv_cache* c, const void* k, long long ld_k,
   VXG_ARG(dtype_known(dtype), "unknown element type %d", dtype);
   if (total == 0 || n_seq == 0) return VXG_OK;
   VXG_ARG(k && v, "NULL input");
+  VXG_ARG(aligned(dtype_bytes(dtype), k, v), "k and v are not aligned to their elements");
   const long long row = (long long)c->heads * c->head_dim;
   VXG_ARG(ld_k >= row && ld_v >= row, "a row stride is below heads * head_dim = %lld", row);
   const long long items = (long long)total / c->page + 2LL * n_seq;

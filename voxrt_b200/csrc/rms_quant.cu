@@ -308,6 +308,8 @@ static vxg_status run(Params p, int dtype, bool norm, cudaStream_t st) {
   VXG_ARG(p.n >= 0 && p.d > 0, "bad shape n=%d d=%d", p.n, p.d);
   if (p.n > 0) VXG_ARG(p.x && (!norm || p.gamma) && (p.q || p.y || p.x_res), "NULL input, or no output given");
   VXG_ARG(!p.q || p.scales, "codes without scales");
+  VXG_ARG(aligned(dtype_bytes(dtype), p.x, p.v, p.x_res, p.y) &&
+              aligned(4, p.gamma, p.scales), "an operand is not aligned to its elements");
   VXG_ARG(!p.q || (p.group > 0 && p.d % p.group == 0), "group %d does not divide the row width %d", p.group, p.d);
   if (!p.q) p.group = p.d;
   VXG_ARG(p.ld_x >= p.d && (!p.v || p.ld_v >= p.d) && (!p.x_res || p.ld_res >= p.d) && (!p.y || p.ld_y >= p.d),
@@ -381,6 +383,7 @@ vxg_status vxg_dequantize_rows(const int8_t* q, const float* scales, int n, int 
   VXG_ARG(n <= 0 || (q && scales && out), "NULL pointer");
   VXG_ARG(dtype_known(dtype), "unknown element type %d", dtype);
   VXG_ARG(n >= 0 && inp > 0 && group > 0 && inp % group == 0, "bad shape n=%d inp=%d group=%d", n, inp, group);
+  VXG_ARG(aligned(dtype_bytes(dtype), out) && aligned(4, scales), "an operand is not aligned to its elements");
   if (n == 0) return VXG_OK;
   const unsigned long long total = (unsigned long long)n * (unsigned)inp;
   const bool vec = group % 16 == 0 && (((uintptr_t)q | (uintptr_t)out) & 15) == 0;
