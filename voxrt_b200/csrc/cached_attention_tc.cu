@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int ppp = 1 << (PL - 4), box = ::min(128, 1 << PL);  // pieces of a page, rows of a copy
     bool ok = true, gone = false;
     float ref = 0.0f;
-    int it = 0;
+    int it = 0, ik = 0, iv = 0;  // blocks; copies of keys and of values begun
     for (Blocks x(p, first); !x.done() && ok; x.next(p), it++) {
       const Tile& t = x.w.t;
       const int key0 = (t.blk0 + x.w.off + x.b) * BK, h = x.w.h;
@@ -192,21 +192,18 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (lane == 0) mbar_arrive_expect_tx(rkfull, bytes);
       __syncwarp();
       if (bring) tma_load_2d(smem + Lay::RK + lane * 16 * HD, &map_k, 0, row, rkfull);
+      ik++;
       if (it > 0 && !wait_phase(rvempty, (it - 1) & 1, p.status, VXG_DEV_TIMEOUT_CACHE_ATTN)) ok = false;
       ok = __all_sync(0xffffffffu, ok);
-      if (!ok) {
-        it++;  // this block's keys are on their way
-        break;
-      }
+      if (!ok) break;
       if (lane == 0) mbar_arrive_expect_tx(rvfull, bytes);
       __syncwarp();
       if (bring) tma_load_2d(smem + Lay::RV + lane * 16 * HD, &map_v, 0, row, rvfull);
+      iv++;
     }
-    // every copy lands before the block may end
-    if (it > 0) {
-      wait_phase(rkfull, (it - 1) & 1, p.status, VXG_DEV_TIMEOUT_DRAIN);
-      if (ok) wait_phase(rvfull, (it - 1) & 1, p.status, VXG_DEV_TIMEOUT_DRAIN);
-    }
+    // every copy lands before the block may end, after a wait that ran out as well
+    if (ik > 0) wait_phase(rkfull, (ik - 1) & 1, p.status, VXG_DEV_TIMEOUT_DRAIN);
+    if (iv > 0) wait_phase(rvfull, (iv - 1) & 1, p.status, VXG_DEV_TIMEOUT_DRAIN);
   } else if (warp >= SOFT_WARPS && warp < MMA_WARP) {
     // ---------------------------------------------------------------------------------------- codes -> operands
     // Eight lanes (16 codes each; four for 64 columns) take a key, a warp four (eight) keys a pass, all in one 16-key piece.
