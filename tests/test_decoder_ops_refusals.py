@@ -232,3 +232,44 @@ def test_operands_across_an_element_boundary():
     assert refused(_write(c, start=P + 2)) and refused(_attend(c, lens=P + 2)) and refused(_read(c, start=P + 2))
     for kw in (dict(k_scales=P + 2), dict(v_scales=P + 1)):
         assert refused(_write(_cache(**kw))) and refused(_attend(_cache(**kw))) and refused(_read(_cache(**kw)))
+
+
+def test_sizes_that_an_int_does_not_hold(monkeypatch):
+    """ctypes cuts a size to 32 bits: 2^32 + 5 rows would become 5, and a window of 2^32 + 5 keys one of 5."""
+    from voxrt_b200 import kernels as K
+
+    most = (1 << 32) + 5
+    wide = lambda *shape: torch.zeros((1,) * len(shape)).expand(shape)
+    calls = []
+    monkeypatch.setattr(KvCache.attend.__globals__["torch"]._C, "_cuda_getDevice", lambda: 0)
+    for m in (K, sys.modules["voxrt_b200.cache"]):
+        monkeypatch.setattr(m, "_call", lambda fn, idx, stream, used, *a: calls.append(a))
+        monkeypatch.setattr(m, "_like", lambda t, shape, dt, stream: torch.empty(shape, dtype=dt))
+        monkeypatch.setattr(m, "_gpu", lambda stream, *t: 0)
+    monkeypatch.setattr(K, "QuantAct", lambda *a: a)
+    a = _Act(1, 16, torch.ones((1, 1)), 16)
+    a.n, a.scales = most, wide(most, 1)
+    w = _Act(8, 16, None, 16)
+    w.w, w.scales, w.out = w.x, torch.ones(8), 8
+    for run in (lambda: K.quantize(wide(most, 16), 16), lambda: K.rms_quant(wide(most, 16), torch.ones(16)),
+                lambda: K.rms_norm(wide(most, 16), torch.ones(16), wide(most, 16)), lambda: K.dequantize(a),
+                lambda: K.gemm_i8(w, a, wide(most, 8))):
+        with pytest.raises(ValueError, match="size of 4294967301"):
+            run()
+    c = KvCache.__new__(KvCache)
+    c.k = c.v = c.ks = c.vs = torch.zeros(1)
+    c.heads, c.head_dim, c.page, c.n_pages, c._ref, c._ws_bytes = 2, 64, 16, 8, None, {}
+    ints = lambda *shape: torch.zeros((1,) * len(shape), dtype=torch.int32).expand(shape).contiguous()
+    table, lens, cu = ints(1, 4), ints(1), ints(2)
+    for run in (lambda: c.write(wide(most, 2, 64), wide(most, 2, 64), table, lens, cu), lambda: c.read(table, lens, cu, most),
+                lambda: c.attend(wide(most, 2, 64), table, lens, cu)):
+        with pytest.raises(ValueError, match="size of 4294967301"):
+            run()
+    assert not calls
+    q = torch.zeros((1, 2, 64))
+    for window, want in ((0, 0), (7, 7), (most, 0x7FFFFFFF)):
+        c.attend(q, table, lens, cu, window=window)
+        assert calls.pop()[13] == want
+    for window in (-1, -most + 5):
+        with pytest.raises(ValueError, match="negative"):
+            c.attend(q, table, lens, cu, window=window)

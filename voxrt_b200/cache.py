@@ -8,7 +8,7 @@ import ctypes as C
 import torch
 
 from ._lib import lib
-from .kernels import _DTYPES, _call, _dt, _gpu, _like
+from .kernels import _DTYPES, _call, _dt, _fits, _gpu, _like
 
 
 class _Desc(C.Structure):  # vxg_kv_cache
@@ -21,6 +21,7 @@ def _stacked(t: torch.Tensor, heads: int, hd: int, what: str) -> int:
     shape = t.shape
     if len(shape) != 3 or shape[1] != heads or shape[2] != hd:
         raise ValueError(f"{what} has shape {tuple(shape)}, not (rows, {heads}, {hd})")
+    _fits(shape[0])
     if t.is_contiguous():
         return heads * hd
     if t.stride(2) != 1 or (heads > 1 and t.stride(1) != hd):
@@ -64,6 +65,7 @@ class KvCache:
         if a.shape != (n_seq,) or cu.shape != (n_seq + 1,):
             raise ValueError(f"page table {tuple(table.shape)}, lengths {tuple(a.shape)} and offsets {tuple(cu.shape)} do "
                              "not belong to one batch")
+        _fits(n_seq, width)
         return idx, n_seq, width
 
     def write(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, start: torch.Tensor, cu: torch.Tensor,
@@ -86,6 +88,7 @@ class KvCache:
         idx, n_seq, width = self._batch(table, start, cu, stream)
         if dtype not in _DTYPES:
             raise ValueError(f"element type {dtype} is none of float16, bfloat16, float32")
+        _fits(total)
         shape = (total, self.heads, self.head_dim)
         k, v = _like(self.k, shape, dtype, stream), _like(self.k, shape, dtype, stream)
         _call(lib().vxg_cache_read, idx, stream, (table, start, cu, self.k, self.v, self.ks, self.vs), self._ref,
@@ -107,6 +110,8 @@ class KvCache:
         heads, hd = q.shape[1] if q.dim() == 3 else 0, self.head_dim
         if heads == 0 or heads % self.heads != 0:
             raise ValueError(f"{heads} query heads for {self.heads} key / value heads")
+        if window < 0:
+            raise ValueError("window must not be negative")
         dt, ld_q = _dt(q), _stacked(q, heads, hd, "q")
         if out is None:
             out = _like(q, q.shape, q.dtype, stream)
@@ -123,6 +128,6 @@ class KvCache:
         ws = _like(q, (nb,), torch.uint8, stream)
         _call(lib().vxg_cache_attention, idx, stream, (q, table, lengths, cu, out, self.k, self.v, self.ks, self.vs),
               self._ref, q.data_ptr(), ld_q, heads, dt, total, table.data_ptr(), n_seq, width, lengths.data_ptr(),
-              cu.data_ptr(), scale if scale is not None else hd ** -0.5, causal, window, out.data_ptr(), ld_out,
+              cu.data_ptr(), scale if scale is not None else hd ** -0.5, causal, min(window, 0x7FFFFFFF), out.data_ptr(), ld_out,
               ws.data_ptr(), nb)
         return out

@@ -52,8 +52,15 @@ def _dt(t: torch.Tensor) -> int:
     return code
 
 
+def _fits(*sizes: int) -> None:
+    """Sizes go to the C entries as int, which ctypes would cut to 32 bits without a word."""
+    if max(sizes) > 0x7FFFFFFF:
+        raise ValueError(f"a size of {max(sizes)} is more than the entries take (2^31 - 1)")
+
+
 def _rows(t: torch.Tensor, n: int, d: int, what: str) -> int:
     """Row stride in elements of an [n, d] operand whose rows are contiguous."""
+    _fits(n, d)
     if t.shape != (n, d):
         raise ValueError(f"{what} has shape {tuple(t.shape)}, not {(n, d)}")
     if t.is_contiguous():
@@ -241,6 +248,7 @@ def quantize(x: torch.Tensor, group: int = GROUP, stream=None) -> QuantAct:
 
 def _scales_of(x: QuantAct) -> torch.Tensor:
     """x's scales, one for each of its groups: the kernels read that many."""
+    _fits(x.n, x.inp, x.group)
     if x.group <= 0 or x.inp % x.group != 0 or x.scales.numel() != x.n * (x.inp // x.group):
         raise ValueError(f"{x.scales.numel()} scales for {x.n} rows of width {x.inp} in groups of {x.group}")
     return x.scales
@@ -286,6 +294,7 @@ def rms_quant(x: torch.Tensor, gamma: torch.Tensor, group: int | None = None, ep
     if x.dim() != 2 or x.shape[1] == 0:
         raise ValueError("x must be [n, d]")
     n, d = x.shape
+    _fits(n, d)
     group = d if group is None else int(group)
     if group <= 0 or d % group != 0:
         raise ValueError(f"group {group} does not divide the row width {d}")
