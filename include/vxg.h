@@ -216,7 +216,7 @@ vxg_status vxg_cache_read(const vxg_kv_cache* c, const int* table, int n_seq, in
 /* Attention of the stacked queries over their sequences' cached tokens: out = softmax(scale * q k^T) v with len[s]
  * (device int32) tokens in the cache, new ones included; query i of n sits at position len - n + i and sees positions
  * < len, <= its own if causal, and > its own - window if window > 0; a query that sees none gives 0. scale is any
- * finite number, negative ones included. q and out: rows
+ * number up to 2^127 in size, negative ones included. q and out: rows
  * [heads * head_dim] of `dtype` with strides ld_q, ld_out, rows 16-byte aligned; heads is a multiple of the cache's
  * heads and query head h reads cache head h / (heads / cache heads). workspace: device memory of
  * vxg_cache_attention_workspace_bytes(), 16-byte aligned, one per call in flight (calls that may overlap, captured

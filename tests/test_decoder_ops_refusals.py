@@ -105,6 +105,14 @@ def test_write_read_attend():
     assert L.vxg_cache_attention_workspace_bytes(4, 1, 4, 2, 64, 2) > 0
 
 
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), float("-inf"), 2.4e38, -3e38])
+def test_scales_beyond_the_kernels_range(scale):
+    """The kernels take the scale times log2(e), which an accepted 3e38 turned into infinity."""
+    assert _attend(_cache(), scale=scale) == ARG and b"scale" in _lib.lib().vxg_last_error()
+    if abs(scale) < 1e39:
+        assert _attend(_cache(), scale=scale / 2, nb=16) == ARG and b"workspace" in _lib.lib().vxg_last_error()
+
+
 def test_python_refusals():
     x = torch.zeros((2, 64))
     with pytest.raises(ValueError, match="CUDA"):

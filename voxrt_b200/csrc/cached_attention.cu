@@ -394,7 +394,8 @@ vxg_status vxg_cache_attention(const vxg_kv_cache* c, const void* q, long long l
   VXG_ARG(dtype_known(dtype), "unknown element type %d", dtype);
   VXG_ARG(heads > 0 && heads % c->heads == 0, "%d query heads for %d key / value heads", heads, c->heads);
   VXG_ARG(window >= 0, "window must not be negative");
-  VXG_ARG(scale == scale && scale - scale == 0.0f, "scale must be finite");
+  const float scale_log2 = scale * 1.44269504088896340736f;
+  VXG_ARG(scale_log2 - scale_log2 == 0.0f, "scale, and its product with log2(e), must be finite");
   if (total == 0 || n_seq == 0) return VXG_OK;
   VXG_ARG(q && out && workspace, "NULL pointer");
   const long long row = (long long)heads * c->head_dim, eb = (long long)dtype_bytes(dtype);
@@ -414,7 +415,7 @@ vxg_status vxg_cache_attention(const vxg_kv_cache* c, const void* q, long long l
   p.status = status, p.n_seq = n_seq, p.max_pages = max_pages, p.total = total, p.heads = heads;
   p.share = heads / c->heads, p.window = window, p.causal = causal != 0, p.slots = pl.slots, p.grid = pl.grid;
   for (p.page_log2 = 4; 1 << p.page_log2 < c->page;) p.page_log2++;
-  p.scale_log2 = scale * 1.44269504088896340736f;
+  p.scale_log2 = scale_log2;
   cudaStream_t st = (cudaStream_t)stream;
   if (pl.mt == 256) return catt::launch_tc(p, pl, c->head_dim, dtype, st);
   if (pl.mt <= 16) return catt::launch_few(p, pl, c->head_dim, dtype, st);
