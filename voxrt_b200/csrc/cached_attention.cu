@@ -299,34 +299,34 @@ __global__ void __launch_bounds__(THREADS, 2)
     const bool whole = off == 0 && take == t.cost;
     float* part = p.part + ((size_t)blockIdx.x * MAX_PIECES + (w.first ? 0 : 1)) * MT * (HD + 2);
     // thread (g, c)'s columns: HD / 4 consecutive ones, the first HD / 8 in o[.][0 or 2], the rest in o[.][1 or 3]
-    #pragma unroll
-          for (int e = 0; e < 2; e++) {
-            const int r = row0 + g + 8 * e;
-            if (r >= t.rows) continue;
-            if (whole) {
-              const int rr = t.r0 + r;
-              T* o = static_cast<T*>(p.out) + (long long)(t.q0 + rr / p.share) * p.ld_out +
-                     (long long)(h * p.share + rr % p.share) * HD + c * (HD / 4);
-              const float inv = S.l[e] == 0.0f ? 0.0f : unit / S.l[e];
-    #pragma unroll
-              for (int j = 0; j < HD / 8; j += 8) {
-                float a[8], b2[8];
-    #pragma unroll
-                for (int k = 0; k < 8; k++) a[k] = S.o[j + k][2 * e] * inv * S.ref, b2[k] = S.o[j + k][2 * e + 1] * inv * S.ref;
-                store8<DT>(o + j, a);
-                store8<DT>(o + HD / 8 + j, b2);
-              }
-            } else {
-              float* o = part + r * (HD + 2);
-              if (c == 0) o[0] = S.m[e], o[1] = S.l[e];
-              o += 2 + c * (HD / 4);
-    #pragma unroll
-              for (int j = 0; j < HD / 8; j++) {
-                o[j] = S.o[j][2 * e] * unit * S.ref;
-                o[HD / 8 + j] = S.o[j][2 * e + 1] * unit * S.ref;
-              }
-            }
-          }
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      const int r = row0 + g + 8 * e;
+      if (r >= t.rows) continue;
+      if (whole) {
+        const int rr = t.r0 + r;
+        T* o = static_cast<T*>(p.out) + (long long)(t.q0 + rr / p.share) * p.ld_out +
+               (long long)(h * p.share + rr % p.share) * HD + c * (HD / 4);
+        const float inv = S.l[e] == 0.0f ? 0.0f : unit / S.l[e];
+#pragma unroll
+        for (int j = 0; j < HD / 8; j += 8) {
+          float a[8], b2[8];
+#pragma unroll
+          for (int k = 0; k < 8; k++) a[k] = S.o[j + k][2 * e] * inv * S.ref, b2[k] = S.o[j + k][2 * e + 1] * inv * S.ref;
+          store8<DT>(o + j, a);
+          store8<DT>(o + HD / 8 + j, b2);
+        }
+      } else {
+        float* o = part + r * (HD + 2);
+        if (c == 0) o[0] = S.m[e], o[1] = S.l[e];
+        o += 2 + c * (HD / 4);
+#pragma unroll
+        for (int j = 0; j < HD / 8; j++) {
+          o[j] = S.o[j][2 * e] * unit * S.ref;
+          o[HD / 8 + j] = S.o[j][2 * e + 1] * unit * S.ref;
+        }
+      }
+    }
     w.next(p, MT, BK);
   }
 }
@@ -412,8 +412,8 @@ vxg_status vxg_cache_attention(const vxg_kv_cache* c, const void* q, long long l
   p.c = *c, p.q = q, p.out = out, p.ld_q = ld_q, p.ld_out = ld_out, p.table = table, p.len = len, p.cu = cu;
   p.rec = static_cast<long long*>(workspace);
   p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.rec_bytes);
-  p.status = status, p.n_seq = n_seq, p.max_pages = max_pages, p.total = total, p.heads = heads;
-  p.share = heads / c->heads, p.window = window, p.causal = causal != 0, p.slots = pl.slots, p.grid = pl.grid;
+  p.status = status, p.n_seq = n_seq, p.max_pages = max_pages, p.total = total;
+  p.share = heads / c->heads, p.window = window, p.causal = causal != 0, p.slots = pl.slots;
   for (p.page_log2 = 4; 1 << p.page_log2 < c->page;) p.page_log2++;
   p.scale_log2 = scale_log2;
   cudaStream_t st = (cudaStream_t)stream;
