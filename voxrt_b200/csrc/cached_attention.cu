@@ -9,8 +9,9 @@
 // power of two, `scale` and log2(e) multiply the f32 sum. The softmax is kept in f32 with a running sum and a reference
 // that may lag behind the maximum by up to 2^8, so that it seldom moves; a probability enters the second product as
 // f16(p * 2^7 * v_scale / ref), ref being the largest value scale met so far (rounding 2^-11 of each term at most, 2^-32
-// absolute against the largest; two parts for f32), and ref and 2^-7 multiply the result. The sum of the row is taken
-// from the unrounded p.
+// absolute against the largest; two parts for f32, 2^-22), which costs digits where p * v_scale falls below 2^-21 of ref
+// (f32: 2^-10), as in a page whose scale is that much smaller than another's; ref and 2^-7 multiply the result. The sum of
+// the row is taken from the unrounded p.
 //
 // Work split. A tile is MT consecutive (query, query head) rows of one sequence and KV head, so a key is read once for
 // all the query heads that share it. The keys it sees, in blocks of 64, times all tiles and KV heads form one line of
@@ -166,7 +167,8 @@ __global__ void __launch_bounds__(THREADS, 2)
 
     const int nb = t.nblk > 0 ? take : 0;
     float inv_ref = 0.0f;
-    // 32 keys of a block: what fits the registers beside O and Q
+    // 32 keys of a block: what fits the registers beside O and Q for heads of 64. f32 queries over heads of 128 spill some
+    // 850 bytes a thread here (4 x 1024 queries over 1000, 16 heads: 553 us).
     auto keys32 = [&](auto tag, const uint8_t* kt, const uint8_t* vt, const float* scales, int key0) {
       constexpr bool masked = decltype(tag)::value;
       // ---- scores. 16-bit queries: the codes enter as 1152 + code, and the sums begin at -1152 times the row's sum

@@ -7,7 +7,8 @@
 // word. Keys enter as 1152 + code, an f16 that needs no subtraction, and the sums begin at -1152 times the query row's sum
 // (f32 queries, which need more than 16 bits of it, subtract). P^T comes out of S^T by an 8 x 8 transpose within the warp.
 // The warps' states meet in shared memory at the end of a piece. Measured: 64 ragged sequences over up to 16000 tokens, 8
-// cache heads of 128 for 32 query heads, 241 us (1.28 GB, 5.3 TB/s); f32 queries 318 us; one sequence over 1500 tokens, 16
+// cache heads of 128 for 32 query heads, 241 us (1.28 GB, 5.3 TB/s); f32 queries 312 us (4.1 TB/s); 16 heads of 64 without
+// sharing 289 us (4.4 TB/s); 16-row tiles, 16 x 4 queries over 4000, 63 us (2.1 TB/s); one sequence over 1500 tokens, 16
 // heads of 64, 12 us, the chain of dependent loads of the two kernels for the most part.
 #include <cuda_runtime.h>
 

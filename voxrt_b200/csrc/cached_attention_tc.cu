@@ -14,10 +14,13 @@
 // TMEM (512 columns): scores of a half at 128 half and 64 columns on, O at 256 + HD half. A step's scores overwrite the
 // probabilities of the step before last: the tensor cores run one thread's products in order.
 //
-// Bound by the softmax warps, of which registers and TMEM allow two a scheduler: per 128 keys and 256 rows the tensor
-// cores need 2048 clocks (measured alone) and the exponentials as many (16 a clock); the kernel takes about 5800 with its
-// pieces' ends (4 ragged sequences of up to 2048 queries of 32 heads behind up to 2000 cached tokens: 389 us, 520 TFLOP/s of
-// what is visible). Slower: longer unrolled loops (instruction fetches of four roles), one pass over scores held in
+// Bound by the softmax warps, of which registers and TMEM allow two a scheduler, and by the pieces' ends, which are serial
+// (the last product, the result, the next Q, the first product): per 128 keys and 256 rows the tensor cores need 2048
+// clocks (measured alone) and the exponentials as many (16 a clock). Measured, 4 sequences of 2048 queries, 32 heads over
+// 8: behind 4096, 8192 and 16384 tokens 806, 1377 and 2742 us, 2.6 to 3.1 us for a further block of 128 keys of a CTA; behind
+// none 507 us, where the CTAs with the first queries' tiles have some 36 pieces of one to three blocks each, by which a
+// piece's end costs about 10 us (inferred). 4 ragged sequences of up to 2048 queries behind up to 2000: 404 us, 500
+// TFLOP/s of what is visible. Slower: longer unrolled loops (instruction fetches of four roles), one pass over scores held in
 // registers. No gain: sixteen softmax warps of half rows, a quarter of the exponentials by polynomial.
 #include <cuda_runtime.h>
 

@@ -7,7 +7,8 @@
 // warps share the K axis, and the weights go from memory straight into the operand registers of mma.m16n8k32: the words of a
 // thread's 16-byte load of a channel are its k slots of two steps, and as the token operand is loaded in the same order the
 // permutation of k cancels. The warps' partial sums meet in shared memory. Measured: one token, 16384 x 8192 weights
-// (larger than L2) 23.7 us, 5.7 TB/s; 4096 x 4096 (in L2) 4.9 us; 37 tokens, 8192 x 2048, 7.1 us.
+// (larger than L2) 24 to 27 us, 5.0 to 5.7 TB/s; 37 tokens, 16384 x 8192 41 us (3.3 TB/s); 8192 x 2048 with three and four
+// sets of operands in turn (50 and 67 MB, in L2 for a part) 7.1 and 9.0 us.
 #include <cuda_runtime.h>
 
 #include <algorithm>

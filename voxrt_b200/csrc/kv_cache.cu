@@ -11,7 +11,8 @@
 // Bound by memory for long runs, by the chain of dependent loads (offsets, page table, values) for single tokens: one
 // block takes one page of K or V and a run of heads, finds its sequence with 32 probes a step, and holds a head's new values
 // in registers between the maximum and the codes, with the next head's on their way. Measured: 64 sequences of one token
-// 5.3 us; 8 ragged sequences of up to 2048 tokens, 8 heads of 128, 24.6 us (100 MB, 4 TB/s), read back 20.8 us (5.2 TB/s).
+// 5.5 us; 8 ragged sequences of up to 2048 tokens, 8 heads of 128, 24.7 us (79 MB, 3.2 TB/s), read back 21.0 us (80 MB,
+// 3.8 TB/s).
 #include <cuda_runtime.h>
 
 #include <algorithm>

@@ -4,15 +4,18 @@
 //   per group: a = max|y|, s = a / 127 (1 if a = 0), code = clamp(round_ties_even(y * (1/s)), +-127)
 //
 // The sum of squares and 1/sqrt run in 64 bits and are rounded once. A 24-bit square is exact there and the sum's own
-// error is below 2^-45, so the codes do not depend on how a row is split over threads, and a row gives the same codes
-// whatever kernel shape it is computed with. Scale and code are the quantiser's of the other entries (quant_scale,
+// error is below 2^-45, so that how a row is split over threads (by the number of rows, among others) shows in its root
+// only where that lies within 2^-45 of the middle between two f32 values: in fewer than one row in a million by this
+// bound. Scale and code are the quantiser's of the other entries (quant_scale,
 // quant_code: a NaN gives code 0 and is skipped by the maximum).
 //
 // Bound by memory: x and v are read once, the sum, the codes and the normalised row written once, and a row stays in
-// registers (eight elements a thread and vector) between the two reductions. A row of up to 256 elements belongs to
-// one warp, a longer one to a block. Measured: 16384 x 4096 bf16 with residual 102 us (470 MB, 4.6 TB/s), 8192 x 4096 f32
-// 87 us (5.0 TB/s), one row of 1024 2.9 us. 16-bit rows are held below the copy rate by issue (68 % of the slots busy):
-// with the squares summed in f32 the first would take 97 us, the second is the same.
+// registers (eight elements a thread and vector) between the two reductions: all of it with up to four vectors a thread.
+// With eight, beside the next row's, 330 (16-bit) to 1030 bytes (f32) a thread spill: 4096 x 16384 f32 takes 346 us,
+// 2.5 TB/s. A row of up to 256 elements belongs to one warp, a longer one to a block. Measured: 16384 x 4096 bf16 with
+// residual 100 us (470 MB, 4.7 TB/s), 16384 x 1024 f16 31 us (3.8 TB/s), 8192 x 4096 f32 86 us (5.1 TB/s), one row of 1024
+// 2.8 us. Without the codes and the residual 16384 x 4096 takes 58 us, the quantiser alone 41. 16-bit rows are held below the copy rate by issue (68 % of the slots busy):
+// with the squares summed in f32 the first would take 5 % less, f32 rows the same.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -55,8 +58,8 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
-// 1 / sqrt(v) in 64 bits, rounded to 32: from a 32-bit root y, with e = 1 - v y^2 below 2^-21, the series
-// y (1 + e / 2 + 3 e^2 / 8) leaves 5 e^3 / 16, less than a 64-bit rounding. Outside f32's range the library's operations.
+// 1 / sqrt(v) in 64 bits, rounded to 32, by one step of Householder's third-order method: from a 32-bit root y, with
+// e = 1 - v y^2 below 2^-21, the series y (1 + e / 2 + 3 e^2 / 8) leaves 5 e^3 / 16, less than a 64-bit rounding. Outside f32's range the library's operations.
 __device__ __forceinline__ float inv_root(double v) {
   if (!(v > 1e-36 && v < 1e37)) return (float)__ddiv_rn(1.0, __dsqrt_rn(v));
   const double y = (double)rsqrtf((float)v);
