@@ -90,6 +90,12 @@ def test_bad_batch(kw, want):
     assert _write(c, **kw) == want and _attend(c, **kw) == want and _read(c, **kw) == want
 
 
+def test_batches_of_too_many_sequences():
+    for n_seq in ((1 << 30) + 1, 0x7FFFFFFF):
+        for call in (_write, _attend, _read):
+            assert call(_cache(), n_seq=n_seq) == UNSUP and b"sequences" in _lib.lib().vxg_last_error()
+
+
 def test_write_read_attend():
     c = _cache()
     for kw in (dict(k=None), dict(v=None), dict(ldk=127), dict(ldv=1), dict(start=None)):

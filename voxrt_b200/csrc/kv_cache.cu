@@ -271,8 +271,8 @@ vxg_status cache_batch_check(const vxg_kv_cache* c, const int* table, int n_seq,
           total);
   VXG_ARG(n_seq == 0 || total == 0 || (table && a && cu && max_pages > 0), "NULL page table, lengths or offsets");
   VXG_ARG(aligned(4, table, a, cu), "page table, lengths and offsets must be 4-byte aligned");
-  if ((long long)max_pages * c->page > 0x7FFFFF00LL) {
-    set_error("sequences of %d pages of %d tokens not supported", max_pages, c->page);
+  if ((long long)max_pages * c->page > 0x7FFFFF00LL || n_seq > (1 << 30)) {  // 32 probes a step pass 31 bits beyond
+    set_error("%d sequences of %d pages of %d tokens not supported", n_seq, max_pages, c->page);
     return VXG_ERR_UNSUPPORTED;
   }
   return VXG_OK;
