@@ -210,6 +210,34 @@ def test_pages_out_of_range_are_masked(KvCache, hd, heads, new, page, dtype):
         assert (np.abs(got - want) <= bound).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hd,heads,new", [(64, 2, 3), (128, 2, 7), (64, 2, 30), (128, 2, 30), (64, 2, 150), (128, 2, 150)])
+def test_pages_out_of_range_under_other_extremes(KvCache, hd, heads, new, dtype):
+    """A negative scale beside such pages, scale 0, and NaN and infinite queries that see no other page, which give 0 like
+    any query that sees no key."""
+    from voxrt_b200._lib import device_status
+
+    rng = np.random.default_rng(hd + new)
+    lens = [200, 200]
+    table, n_pages = _table(rng, lens, 32)
+    ref, c = _pair(KvCache, rng, n_pages, 1, 32, hd)
+    ref.scales[0] *= np.float32(0.02)
+    c.ks.copy_(torch.from_numpy(ref.scales[0]))
+    bad = table.copy()
+    bad[0, [1, 4, 6]] = n_pages
+    bad[1, :7] = -1
+    hidden = [(0, 1), (0, 4), (0, 6)] + [(1, i) for i in range(7)]
+    cu = [0, new, 2 * new]
+    q = torch.from_numpy(rng.standard_normal((2 * new, heads, hd)).astype(np.float32) * 1.5).to(dtype).cuda()
+    finite = f32(q)
+    q[new:, 0, 5], q[new:, 1, 7] = float("nan"), float("inf")
+    for scale in (-0.2, 0.0, 0.2):
+        got = f32(c.attend(q, _int(bad), _int(lens), _int(cu), scale=scale)).astype(np.float64)
+        want, bound = attend(ref, finite, table, lens, cu, float(np.float32(scale)), True, 0, dtype, hidden)
+        assert device_status() == 0x302
+        assert (np.abs(got - want) <= bound).all() and (got[new:] == 0).all()
+
+
 CASES = [  # (page, hd, kv heads, query heads, lengths, new tokens, causal, window)
     (16, 64, 1, 1, [1], [1], True, 0),
     (16, 64, 2, 2, [1, 17, 64, 65, 200], [1, 1, 1, 1, 1], True, 0),

@@ -201,11 +201,11 @@ __global__ void __launch_bounds__(THREADS, 2)
       float mx[2] = {-INFINITY, -INFINITY}, vsm = 0.0f;
 #pragma unroll
       for (int j = 0; j < TOK / 8; j++) {
-        const float ks = scales[j / 2], hide = ks < 0.0f ? -INFINITY : 0.0f;  // NO_PAGE
+        const float ks = scales[j / 2];
         vsm = fmaxf(vsm, scales[4 + j / 2]);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-          float x = __fmaf_rn(s[j][k], rowf[k >> 1] * ks, hide);
+          float x = ks < 0.0f ? -INFINITY : s[j][k] * (rowf[k >> 1] * ks);  // < 0: NO_PAGE
           if (masked) {
             const int key = key0 + 8 * j + 2 * c + (k & 1);
             if (key < klo[k >> 1] || key >= khi[k >> 1]) x = -INFINITY;
