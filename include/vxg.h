@@ -183,7 +183,7 @@ vxg_status vxg_attention_i8(const float* qkv, int ld_qkv, const float* rel_k, in
  * scale per (page, head), all caller-owned device memory; a sequence's pages are listed in order in its row of a page
  * table [n_seq, max_pages] (device int32). page is 16, 32, 64 or 128 tokens, head_dim 64 or 128 (else
  * VXG_ERR_UNSUPPORTED); the codes are 16-byte aligned. Scales start as 0 or anything else: a page's first write sets
- * them. Up to 2^30 sequences of up to 2^31 - 256 tokens. No reference counterpart (its decoder is an LSTM).
+ * them; scales of pages that a caller fills itself are finite and not negative. Up to 2^30 sequences of up to 2^31 - 256 tokens. No reference counterpart (its decoder is an LSTM).
  *
  * A batch is stacked along the token axis like the encoder's: sequence s owns rows [cu[s], cu[s + 1]) of k, v, q and
  * out (cu: device int32 [n_seq + 1], not decreasing, cu[n_seq] <= total; rows behind the last sequence are neither read

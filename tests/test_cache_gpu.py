@@ -401,6 +401,27 @@ def test_scores_that_rise_all_along(KvCache, hd, heads, new, length, dtype):
     assert (np.abs(got - want) <= bound).all()
 
 
+@pytest.mark.parametrize("dtype,hd,heads,new", [(torch.float32, 64, 2, 3), (torch.bfloat16, 128, 2, 7),
+                                               (torch.float32, 128, 2, 30), (torch.float16, 64, 2, 30)])
+def test_small_tiles_take_key_scales_of_either_sign(KvCache, dtype, hd, heads, new):
+    """A write leaves no negative scale, but codes and scales may come from elsewhere; only an id out of range masks."""
+    rng = np.random.default_rng(hd + new)
+    table, n_pages = _table(rng, [200], 16)
+    ref, c = _pair(KvCache, rng, n_pages, 1, 16, hd)
+    ref.scales[0] *= (0.02 * np.where(rng.random(ref.scales[0].shape) < 0.5, -1, 1)).astype(np.float32)
+    c.ks.copy_(torch.from_numpy(ref.scales[0]))
+    q = torch.from_numpy(rng.standard_normal((new, heads, hd)).astype(np.float32)).to(dtype).cuda()
+    got = f32(c.attend(q, _int(table), _int([200]), _int([0, new]), scale=0.11)).astype(np.float64)
+    oracle = Cache(n_pages, 1, 16, hd)  # the same keys as codes of the other sign, for the bound's sake
+    oracle.codes, oracle.scales = [a.copy() for a in ref.codes], [a.copy() for a in ref.scales]
+    flip = (oracle.scales[0] < 0)[:, :, None, None]
+    oracle.codes[0] = np.where(flip, -oracle.codes[0], oracle.codes[0])
+    oracle.scales[0] = np.abs(oracle.scales[0])
+    want, bound = attend(oracle, f32(q), table, [200], [0, new], float(np.float32(0.11)), True, 0, dtype)
+    _ok()
+    assert (np.abs(got - want) <= bound).all()
+
+
 def test_shared_pages_other_stream_and_graph(KvCache):
     """Two sequences over the same prefix pages; a captured call replayed with other lengths; a side stream."""
     rng = np.random.default_rng(10)

@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(THREADS, 2)
         vsm = fmaxf(vsm, scales[4 + j / 2]);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-          float x = ks < 0.0f ? -INFINITY : s[j][k] * (rowf[k >> 1] * ks);  // < 0: NO_PAGE
+          float x = ks == NO_PAGE ? -INFINITY : s[j][k] * (rowf[k >> 1] * ks);
           if (masked) {
             const int key = key0 + 8 * j + 2 * c + (k & 1);
             if (key < klo[k >> 1] || key >= khi[k >> 1]) x = -INFINITY;

@@ -3,6 +3,8 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include <limits>
+
 #include "common.h"
 #include "dtype.cuh"
 #include "kv_cache.cuh"
@@ -36,8 +38,8 @@ struct Plan {
   size_t rec_bytes, part_bytes;
 };
 
-// Stands for the key scale of a page whose id is out of range: its keys take no part. A written page's is not negative.
-constexpr float NO_PAGE = -1.0f;
+// Stands for the key scale of a page whose id is out of range: its keys take no part.
+constexpr float NO_PAGE = -std::numeric_limits<float>::infinity();
 
 constexpr int FEW_CTAS_8 = 3;  // CTAs an SM, tiles of up to 8 rows
 // Tiles of up to 16 rows (cached_attention_few.cu).

@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? FEW_CTAS_8 : 2)
         for (int k = 0; k < 4; k++) {
           const int e = k & 1;
           s[n][k] = (s[n][k] + s2[n][k]) * (rowf[n][e] * ks);
-          if (ks < 0.0f) s[n][k] = -INFINITY;  // NO_PAGE
+          if (ks == NO_PAGE) s[n][k] = -INFINITY;
           if (masked) {
             const int key = key0 + (k >> 1) * 8;
             if (key < klo[n][e] || key >= khi[n][e]) s[n][k] = -INFINITY;

@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 make_uint4(h[0], h[1], h[2], h[3]);
           }
         }
-        // not 0, so that NO_PAGE times infinity is one; below f32's range the scores are alike in any case
+        // not 0, which NO_PAGE would turn into NaN; below f32's range the scores are alike in any case
         const float rowf = fmaxf(__int_as_float((127 - ex) << 23) * p.scale_log2, 1.4e-45f);
         fence_proxy_async_smem();
         tc_fence_before();
@@ -443,7 +443,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (__float_as_int(ref) < 0) {  // scores that NO_PAGE takes to -inf, whatever the query
 #pragma unroll 1
             for (int g = 0; g < SB / 16; g++)
-              if (ks[g] < 0.0f) tmem_st16_const(S + 16 * g, __float_as_uint(INFINITY));
+              if (ks[g] == NO_PAGE) tmem_st16_const(S + 16 * g, __float_as_uint(INFINITY));
             tmem_wait_st();
           }
           // ---- the step's maximum
